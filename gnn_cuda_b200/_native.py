@@ -20,6 +20,7 @@ GNN_ERR_UNSUPPORTED = 3
 GNN_AGG_GCN, GNN_AGG_SUM, GNN_AGG_MEAN, GNN_AGG_MEAN_RECIPROCAL = 0, 1, 2, 3
 GNN_INDEX_INT32, GNN_INDEX_INT64 = 0, 1
 GNN_PRECISION_TF32, GNN_PRECISION_FP32 = 0, 1
+GNN_ROWS_FP32, GNN_ROWS_INT8 = 0, 1
 
 _lib = None
 _lock = threading.Lock()
@@ -76,6 +77,11 @@ PROTOTYPES: dict[str, tuple[object, list[object]]] = {
     "gnn_bias_relu_forward": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp]),
     "gnn_tensor_add_inplace": (_i32, [_vp, _vp, _f32, _i64, _vp]),
     "gnn_relu_inplace": (_i32, [_vp, _i64, _vp]),
+    "gnn_quantize_rows": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "gnn_quantize_weight": (_i32, [_vp, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "gnn_linear_int8_workspace_bytes": (_sz, [_vp, _i32, _i64, _vp, _i64, _i32, _i64, _i64, _i64]),
+    "gnn_linear_int8_forward": (
+        _i32, [_vp, _i32, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _sz, _vp]),
     "gnn_managed_alloc": (_i32, [_sz, _i32, ctypes.POINTER(_vp)]),
     "gnn_managed_free": (_i32, [_vp, _i32]),
     "gnn_hmm_supported": (_i32, [_i32, ctypes.POINTER(_i32)]),

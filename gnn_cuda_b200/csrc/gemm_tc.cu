@@ -31,6 +31,7 @@
 
 #include "common.cuh"
 #include "tc_core.cuh"
+#include "tma_host.cuh"
 
 namespace gnnb200 {
 namespace {
@@ -312,37 +313,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 // host side
 // ---------------------------------------------------------------------------
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess) {
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-    } else {
-      cudaGetLastError();
-    }
-  });
-  return fn;
-}
-
-bool device_is_sm100() {
-  int dev = 0, major = 0, minor = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) {
-    cudaGetLastError();
-    return false;
-  }
-  cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-  cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
-  return major == 10 && minor == 0;
-}
-
 int pick_bn(int64_t n) {
   if (n % 128 == 0) return 128;
   if (n == 64) return 64;
@@ -489,15 +459,17 @@ int tc_status_read(int reset, int* status) {
 
 namespace gnnb200 {
 int spmm_status_read(int reset, int* status);  // spmm.cu
+int i8_status_read(int reset, int* status);    // linear_i8.cu
 }
 
 extern "C" int gnn_device_status(int reset, int* status) {
   GNN_REQUIRE(status != nullptr, GNN_ERR_NULL_POINTER, "status must not be NULL");
-  int tc = 0, sp = 0;
+  int tc = 0, sp = 0, i8 = 0;
   int rc = gnnb200::tc_status_read(reset, &tc);
   if (rc == GNN_OK) rc = gnnb200::spmm_status_read(reset, &sp);
+  if (rc == GNN_OK) rc = gnnb200::i8_status_read(reset, &i8);
   if (rc != GNN_OK) return rc;
-  *status = tc != 0 ? tc : sp;
+  *status = tc != 0 ? tc : (sp != 0 ? sp : i8);
   gnnb200::clear_error();
   return GNN_OK;
 }

@@ -1,0 +1,239 @@
+// fp32 rows to signed 8-bit rows with one scale each (int8_rows.cuh holds the
+// rule), the same for the columns of a weight matrix, and a repack of 8-bit rows
+// whose stride or base does not suit TMA.
+//
+// All three move each byte once. quantize_rows keeps a row's values in registers
+// between the maximum and the rounding (up to 1,024 columns, one warp a row, 4
+// rows of up to 128 columns in flight per warp); wider rows take a block and are
+// read a second time, from L1 / L2.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "int8_rows.cuh"
+
+namespace gnnb200 {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ float warp_max_nan(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max_abs_nan(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+
+// One warp per row, NV * 128 columns at most. VEC: cols % 4 == 0, x 16-byte and q
+// 4-byte aligned, row by row; lane l holds the float4 columns l + 32 j. Otherwise
+// lane l holds the columns l + 32 j, one by one.
+template <int NV, bool VEC>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const float* __restrict__ x, int64_t ldx,
+                                                                 int64_t rows, int cols, int8_t* __restrict__ q,
+                                                                 int64_t ldq, float* __restrict__ scale) {
+  constexpr int R = NV == 1 ? 4 : (NV == 2 ? 2 : 1);  // rows in flight per warp
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  for (int64_t r0 = warp * R; r0 < rows; r0 += warps * R) {
+    float v[R][NV * 4];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float* src = x + (r0 + i) * ldx;
+      const bool live = r0 + i < rows;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if constexpr (VEC) {
+          const int c = (lane + 32 * j) * 4;
+          float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (live && c < cols) t = __ldcs(reinterpret_cast<const float4*>(src + c));
+          v[i][4 * j] = t.x;
+          v[i][4 * j + 1] = t.y;
+          v[i][4 * j + 2] = t.z;
+          v[i][4 * j + 3] = t.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = lane + 32 * (4 * j + e);
+            v[i][4 * j + e] = (live && c < cols) ? __ldcs(src + c) : 0.0f;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (r0 + i >= rows) break;
+      float amax = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NV * 4; ++j) amax = max_abs_nan(amax, v[i][j]);
+      const RowQuant rq = row_quant(warp_max_nan(amax));
+      int8_t* dst = q + (r0 + i) * ldq;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const uint32_t p = quant4(rq, v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2], v[i][4 * j + 3]);
+        if constexpr (VEC) {
+          const int c = (lane + 32 * j) * 4;
+          if (c < cols) *reinterpret_cast<uint32_t*>(dst + c) = p;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = lane + 32 * (4 * j + e);
+            if (c < cols) dst[c] = static_cast<int8_t>((p >> (8 * e)) & 0xffu);
+          }
+        }
+      }
+      if (lane == 0) scale[r0 + i] = rq.s;
+    }
+  }
+}
+
+// One block per row, any width.
+__global__ void __launch_bounds__(kThreads) quantize_wide_rows_kernel(const float* __restrict__ x, int64_t ldx,
+                                                                      int64_t rows, int64_t cols,
+                                                                      int8_t* __restrict__ q, int64_t ldq,
+                                                                      float* __restrict__ scale) {
+  __shared__ float part[kThreads / 32];
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const float* src = x + r * ldx;
+    float amax = 0.0f;
+    for (int64_t c = threadIdx.x; c < cols; c += kThreads) amax = max_abs_nan(amax, __ldg(src + c));
+    amax = warp_max_nan(amax);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
+    __syncthreads();
+    amax = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) amax = max_abs_nan(amax, part[w]);
+    const RowQuant rq = row_quant(amax);
+    for (int64_t c = threadIdx.x; c < cols; c += kThreads) q[r * ldq + c] = quant1(rq, __ldg(src + c));
+    if (threadIdx.x == 0) scale[r] = rq.s;
+    __syncthreads();
+  }
+}
+
+// weight [k, n] -> q [n, k] and one scale per column: 32 columns a block, the
+// maximum over k first, then 32 x 32 tiles turned round through shared memory.
+__global__ void __launch_bounds__(kThreads) quantize_weight_kernel(const float* __restrict__ w, int64_t k, int64_t n,
+                                                                   int8_t* __restrict__ q, int64_t ldq,
+                                                                   float* __restrict__ scale) {
+  __shared__ float red[8][32];
+  __shared__ int8_t tile[32][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + tx;
+  float amax = 0.0f;
+  if (c < n) {
+    for (int64_t r = ty; r < k; r += 8) amax = max_abs_nan(amax, __ldg(w + r * n + c));
+  }
+  red[ty][tx] = amax;
+  __syncthreads();
+  amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = max_abs_nan(amax, red[i][tx]);
+  const RowQuant rq = row_quant(amax);
+  if (ty == 0 && c < n) scale[c] = rq.s;
+  for (int64_t r0 = 0; r0 < k; r0 += 32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t r = r0 + ty + 8 * i;
+      tile[tx][ty + 8 * i] = (c < n && r < k) ? quant1(rq, __ldg(w + r * n + c)) : int8_t(0);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + ty + 8 * i;
+      if (col < n && r0 + tx < k) q[col * ldq + r0 + tx] = tile[ty + 8 * i][tx];
+    }
+    __syncthreads();
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) repack_rows_kernel(const int8_t* __restrict__ x, int64_t ldx, int64_t rows,
+                                                               int64_t cols, int8_t* __restrict__ out, int64_t ldo) {
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); r < rows; r += warps) {
+    for (int64_t c = lane; c < cols; c += 32) out[r * ldo + c] = x[r * ldx + c];
+  }
+}
+
+unsigned grid_for(int64_t units) {
+  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(units, 16LL * sm_count())));
+}
+
+template <int NV>
+void launch_rows(bool vec, const float* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq,
+                 float* scale, cudaStream_t stream) {
+  constexpr int per_block = (NV == 1 ? 4 : (NV == 2 ? 2 : 1)) * (kThreads / 32);
+  const unsigned grid = grid_for((rows + per_block - 1) / per_block);
+  if (vec) {
+    quantize_rows_kernel<NV, true><<<grid, kThreads, 0, stream>>>(x, ldx, rows, static_cast<int>(cols), q, ldq, scale);
+  } else {
+    quantize_rows_kernel<NV, false><<<grid, kThreads, 0, stream>>>(x, ldx, rows, static_cast<int>(cols), q, ldq, scale);
+  }
+}
+
+}  // namespace
+
+int quantize_rows(const float* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq, float* scale,
+                  cudaStream_t stream) {
+  const bool vec = cols % 4 == 0 && ldx % 4 == 0 && ldq % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(q) % 4 == 0;
+  if (cols <= 128) {
+    launch_rows<1>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+  } else if (cols <= 256) {
+    launch_rows<2>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+  } else if (cols <= 512) {
+    launch_rows<4>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+  } else if (cols <= 1024) {
+    launch_rows<8>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+  } else {
+    quantize_wide_rows_kernel<<<grid_for(rows), kThreads, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
+  }
+  GNN_LAUNCH_CHECK("quantize_rows launch");
+  return GNN_OK;
+}
+
+int repack_rows(const int8_t* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* out, int64_t ldo,
+                cudaStream_t stream) {
+  repack_rows_kernel<<<grid_for((rows + 7) / 8), kThreads, 0, stream>>>(x, ldx, rows, cols, out, ldo);
+  GNN_LAUNCH_CHECK("repack_rows launch");
+  return GNN_OK;
+}
+
+}  // namespace gnnb200
+
+using namespace gnnb200;
+
+extern "C" int gnn_quantize_rows(const float* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq,
+                                 float* scale, gnn_stream_t stream) {
+  GNN_REQUIRE(rows >= 0 && cols >= 0, GNN_ERR_INVALID_ARGUMENT, "rows and cols must be >= 0");
+  if (rows == 0) {
+    clear_error();
+    return GNN_OK;
+  }
+  GNN_REQUIRE(scale != nullptr && (cols == 0 || (x != nullptr && q != nullptr)), GNN_ERR_NULL_POINTER,
+              "x, q and scale must not be NULL");
+  GNN_REQUIRE(ldx >= cols && ldq >= cols, GNN_ERR_INVALID_ARGUMENT, "row strides must be >= cols");
+  const int rc = quantize_rows(x, ldx, rows, cols, q, ldq, scale, reinterpret_cast<cudaStream_t>(stream));
+  if (rc == GNN_OK) clear_error();
+  return rc;
+}
+
+extern "C" int gnn_quantize_weight(const float* weight, int64_t k, int64_t n, int8_t* q, int64_t ldq, float* scale,
+                                   gnn_stream_t stream) {
+  GNN_REQUIRE(k >= 0 && n >= 0, GNN_ERR_INVALID_ARGUMENT, "k and n must be >= 0");
+  if (n == 0) {
+    clear_error();
+    return GNN_OK;
+  }
+  GNN_REQUIRE(scale != nullptr && (k == 0 || (weight != nullptr && q != nullptr)), GNN_ERR_NULL_POINTER,
+              "weight, q and scale must not be NULL");
+  GNN_REQUIRE(ldq >= k, GNN_ERR_INVALID_ARGUMENT, "row stride of q must be >= k");
+  GNN_REQUIRE((n + 31) / 32 <= 0x7fffffffLL, GNN_ERR_UNSUPPORTED, "weight too wide");
+  quantize_weight_kernel<<<static_cast<unsigned>((n + 31) / 32), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      weight, k, n, q, ldq, scale);
+  GNN_LAUNCH_CHECK("quantize_weight launch");
+  clear_error();
+  return GNN_OK;
+}

@@ -89,7 +89,7 @@ int gnn_gemm_uses_tensor_cores(int64_t m, int64_t k, int64_t n);
  * segment chain of long rows in the aggregation kernels) give up after ~2 s
  * instead of hanging; they then record a non-zero code here (1-6 tensor-core
  * pipeline, 16 aggregation segment chain, 17 aggregation long-row list
- * overflow) and the kernel moves on. Synchronises with the current device,
+ * overflow, 33-38 8-bit transform pipeline) and the kernel moves on. Synchronises with the current device,
  * stores the word in *status and clears it when reset != 0. */
 int gnn_device_status(int reset, int* status);
 
@@ -278,6 +278,46 @@ int gnn_tensor_add_inplace(float* dst, const float* src, float alpha, int64_t co
 
 /* t = max(t, 0) keeping -0 and NaN as they are. Replaces relu_inplace_cuda_, agg_ops.cu:420. */
 int gnn_relu_inplace(float* t, int64_t count, gnn_stream_t stream);
+
+/* ---- 8-bit rows: quantiser, transform ---------------------------------------- *
+ * No counterpart in the reference, which holds every feature in fp32. A matrix in
+ * signed 8-bit integers has one fp32 scale per row: element (i, j) stands for
+ * q[i, j] * scale[i]. Rows may be strided (ld = elements from row to row); rows
+ * that start on 16-byte boundaries (base and ld multiples of 16) are read as they
+ * are, others are repacked into the workspace first.
+ */
+typedef enum gnn_row_type {
+  GNN_ROWS_FP32 = 0,
+  GNN_ROWS_INT8 = 1 /* signed 8-bit, one fp32 scale per row */
+} gnn_row_type;
+
+/* scale[i] = fp32(max_j |x[i, j]| / 127); q[i, j] = x[i, j] / scale[i] rounded to
+ * the nearest integer, ties to even, decided on the exact quotient. A row of zeros
+ * (or whose scale underflows) has scale 0 and q 0; a row that holds a NaN or an
+ * infinity has scale NaN and q 0. Bytes of q between cols and ldq are not written. */
+int gnn_quantize_rows(const float* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq,
+                      float* scale, gnn_stream_t stream);
+
+/* The columns of weight [k, n] (the layout of gnn_linear_forward) as n rows of k
+ * 8-bit values, one scale per output channel: q is [n, ldq], scale is [n]. */
+int gnn_quantize_weight(const float* weight, int64_t k, int64_t n, int8_t* q, int64_t ldq, float* scale,
+                        gnn_stream_t stream);
+
+/* y = relu?((float(sum_k xq[i, k] * wq[j, k]) * x_scale[i]) * weight_scale[j] + bias[j])
+ * on the tcgen05 tensor cores: the sum is exact (int32, k <= 131071), every later
+ * step is rounded to fp32 in the order written. x is [m, k]: 8-bit rows with
+ * x_scale, or fp32 rows (x_type GNN_ROWS_FP32, x_scale unused), which are quantised
+ * as gnn_quantize_rows does on the way. weight is [n, k] in 8 bits (gnn_quantize_weight).
+ * out is [m, n]: fp32, or 8-bit rows with out_scale [m] (y quantised as
+ * gnn_quantize_rows does). bias may be NULL; out must not overlap an input.
+ * Workspace: gnn_linear_int8_workspace_bytes with the same arguments (0 for aligned
+ * 8-bit x and weight and out fp32 or n <= 256). */
+size_t gnn_linear_int8_workspace_bytes(const void* x, int x_type, int64_t ldx, const int8_t* weight, int64_t ldw,
+                                       int out_type, int64_t m, int64_t k, int64_t n);
+int gnn_linear_int8_forward(const void* x, int x_type, int64_t ldx, const float* x_scale, const int8_t* weight,
+                            int64_t ldw, const float* weight_scale, const float* bias, void* out, int out_type,
+                            int64_t ldo, float* out_scale, int64_t m, int64_t k, int64_t n, int relu,
+                            void* workspace, size_t workspace_bytes, gnn_stream_t stream);
 
 /* ---- one layer in one pass: aggregation + dense transform ------------------- */
 

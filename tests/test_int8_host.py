@@ -1,0 +1,54 @@
+"""Refusals of the 8-bit path that need no device: C entry points and Python checks."""
+import pytest
+import torch
+
+from gnn_cuda_b200 import _native as N
+from gnn_cuda_b200.GNN_cuda_common import int8_ops as I
+
+
+def _linear(m, k, n, x=1 << 20, x_type=1, ldx=None, xs=1 << 20, w=1 << 20, out=1 << 20, out_type=0, ldo=None, os_=None):
+    return N.lib().gnn_linear_int8_forward(x, x_type, k if ldx is None else ldx, xs, w, k, 1 << 20, None, out, out_type,
+                                           n if ldo is None else ldo, os_, m, k, n, 0, None, 0, None)
+
+
+def test_c_entry_refusals():
+    assert _linear(4, 0, 4) == 1 and "k >= 1" in N.last_error()
+    assert _linear(-1, 8, 4) == 1
+    assert _linear(4, 8, 4, x_type=2) == 1 and "row types" in N.last_error()
+    assert _linear(4, 131072, 4) == 3 and "131071" in N.last_error()
+    assert _linear(4, 16, 4, ldx=8) == 1 and "strides" in N.last_error()
+    assert _linear(4, 16, 4, xs=None) == 2 and "x_scale" in N.last_error()
+    assert _linear(4, 16, 4, out_type=1) == 2 and "out_scale" in N.last_error()
+    assert _linear(4, 16, 4, x=None) == 2
+    assert _linear(0, 16, 4) == 0 and _linear(4, 16, 0) == 0
+    L = N.lib()
+    assert L.gnn_quantize_rows(None, 4, 3, 4, None, 4, None, None) == 2
+    assert L.gnn_quantize_rows(1 << 20, 3, 3, 4, 1 << 20, 4, 1 << 20, None) == 1
+    assert L.gnn_quantize_rows(None, 4, 0, 4, None, 4, None, None) == 0
+    assert L.gnn_quantize_weight(None, 4, 3, None, 4, None, None) == 2
+    assert L.gnn_quantize_weight(1 << 20, 8, 3, 1 << 20, 4, 1 << 20, None) == 1
+
+
+def test_workspace_query():
+    q = N.lib().gnn_linear_int8_workspace_bytes
+    al, un = 1 << 20, (1 << 20) + 1
+    assert q(al, 1, 128, al, 128, 0, 1000, 128, 64) == 0
+    assert q(al, 1, 128, al, 128, 1, 1000, 128, 256) == 0
+    assert q(al, 0, 100, al, 112, 0, 1000, 100, 64) >= 1000 * 112 + 4000       # fp32 rows: quantised copy and scales
+    assert q(un, 1, 128, al, 128, 0, 1000, 128, 64) >= 1000 * 128              # unaligned rows: repacked
+    assert q(al, 1, 128, al, 129, 0, 1000, 128, 64) >= 64 * 128
+    assert q(al, 1, 128, al, 128, 1, 1000, 128, 257) >= 4 * 1000 * 257         # wide 8-bit rows: fp32 first
+    assert q(al, 1, 128, al, 128, 0, 0, 128, 64) == 0
+
+
+def test_python_refusals():
+    x8, s = torch.zeros(4, 8, dtype=torch.int8), torch.ones(4)
+    with pytest.raises(RuntimeError, match="q must be CUDA"):
+        I.quantize_rows_(torch.zeros(4, 8), x8, s)
+    with pytest.raises(RuntimeError, match="q must be CUDA"):
+        I.quantize_weight_(torch.zeros(8, 4), x8, s)
+    with pytest.raises(RuntimeError, match="out must be CUDA"):
+        I.linear_int8_forward_(x8, s, x8, s, None, torch.zeros(4, 4))
+    t = I.empty_rows(5, 21, "cpu")
+    assert t.shape == (5, 21) and t.stride(0) == 32
+    assert I._overlap(t, t[2:]) and not I._overlap(t[:2], t[3:])
