@@ -23,7 +23,7 @@ from __future__ import annotations
 import torch
 
 from .. import _native as N
-from .native_ops import _check, _stream
+from .native_ops import _check, _index_type, _stream
 
 
 def empty_rows(rows: int, cols: int, device) -> torch.Tensor:
@@ -168,3 +168,61 @@ def linear_int8_forward_(x: torch.Tensor, x_scale: torch.Tensor | None, weight: 
             xp, x_type, ldx, None if x_scale is None else x_scale.data_ptr(), wp, ldw, weight_scale.data_ptr(), bias_ptr,
             out.data_ptr(), out_type, _ld(out), None if out_scale is None else out_scale.data_ptr(), m, k, n,
             1 if relu else 0, None if ws is None else ws.data_ptr(), wsb, _stream(dev)), "gnn_linear_int8_forward")
+
+
+_WEIGHTING = {"sum": N.GNN_WEIGHT_SUM, "mean": N.GNN_WEIGHT_MEAN, "gcn": N.GNN_WEIGHT_GCN,
+              "weighted": N.GNN_WEIGHT_EDGE}
+
+
+def spmm_int8_forward_(row_ptr: torch.Tensor, col_ind: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor,
+                       out: torch.Tensor, aggregation: str = "sum", deg_inv_sqrt: torch.Tensor | None = None,
+                       edge_weight: torch.Tensor | None = None) -> None:
+    """out[r] = f_r * sum_e w_e * x_scale[c] * x[c] over the entries e = (r, c) of a CSR, in float32.
+
+    aggregation: "sum"; "mean" (divided by the degree); "gcn" (deg_inv_sqrt[r] *
+    deg_inv_sqrt[c]); "weighted" (edge_weight[e]) — the weightings of
+    ``spmm_sum_forward_``, ``spmm_mean_forward_``, ``spmm_gcn_forward_`` and
+    ``spmm_pyg_gcn_forward_``. x: int8 [num_nodes, f] with x_scale [num_nodes]; out:
+    float32 [num_nodes, f]. Rows are summed in another order than the float32
+    aggregations, the same one in every call."""
+    dev = out.device
+    _check(out.is_cuda, "out must be CUDA")
+    _check(aggregation in _WEIGHTING, "aggregation must be sum, mean, gcn or weighted")
+    for name, t in (("row_ptr", row_ptr), ("col_ind", col_ind), ("x", x)):
+        _on_device(name, t, dev)
+    for name, t in (("row_ptr", row_ptr), ("col_ind", col_ind)):
+        _check(t.is_contiguous(), f"{name} must be contiguous")
+        _check(t.dim() == 1, f"{name} must be rank-1")
+    _check(row_ptr.dtype in (torch.int32, torch.int64), "row_ptr must be int32")
+    _check(col_ind.dtype == torch.int32, "col_ind must be int32")
+    _check_rows8("x", x)
+    _check_f32("x_scale", x_scale, 1, dev)
+    _check_f32("out", out, 2, dev)
+    _check(tuple(x.shape) == tuple(out.shape), "x and out must have the same shape")
+    n, f, nnz = x.size(0), x.size(1), col_ind.numel()
+    _check(x_scale.numel() == n, "x_scale length must equal num_nodes")
+    _check(row_ptr.numel() == n + 1, "row_ptr length must be num_nodes + 1")
+    dis_ptr = ew_ptr = None
+    if aggregation == "gcn":
+        _check(deg_inv_sqrt is not None, "deg_inv_sqrt is needed for gcn")
+        _check_f32("deg_inv_sqrt", deg_inv_sqrt, 1, dev)
+        _check(deg_inv_sqrt.numel() == n, "deg_inv_sqrt length must equal num_nodes")
+        dis_ptr = deg_inv_sqrt.data_ptr()
+    else:
+        _check(deg_inv_sqrt is None, "deg_inv_sqrt is only for gcn")
+    if aggregation == "weighted":
+        _check(edge_weight is not None, "edge_weight is needed for weighted")
+        _check_f32("edge_weight", edge_weight, 1, dev)
+        _check(edge_weight.numel() == nnz, "col_ind and edge_weight lengths must match")
+        ew_ptr = edge_weight.data_ptr()
+    else:
+        _check(edge_weight is None, "edge_weight is only for weighted")
+    _check(not _overlap(out, x), "out must not alias x")
+    L = N.lib()
+    with _Device(dev):
+        wsb = L.gnn_spmm_int8_workspace_bytes(n, nnz, f)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        N.check(L.gnn_spmm_int8_forward(
+            row_ptr.data_ptr(), _index_type(row_ptr), col_ind.data_ptr(), _WEIGHTING[aggregation], dis_ptr, ew_ptr,
+            x.data_ptr(), _ld(x), x_scale.data_ptr(), out.data_ptr(), n, nnz, f, ws.data_ptr(), wsb, _stream(dev)),
+            "gnn_spmm_int8_forward")

@@ -21,6 +21,8 @@ GNN_AGG_GCN, GNN_AGG_SUM, GNN_AGG_MEAN, GNN_AGG_MEAN_RECIPROCAL = 0, 1, 2, 3
 GNN_INDEX_INT32, GNN_INDEX_INT64 = 0, 1
 GNN_PRECISION_TF32, GNN_PRECISION_FP32 = 0, 1
 GNN_ROWS_FP32, GNN_ROWS_INT8 = 0, 1
+GNN_ACT_NONE, GNN_ACT_RELU, GNN_ACT_SILU, GNN_ACT_GELU = 0, 1, 2, 3
+GNN_WEIGHT_SUM, GNN_WEIGHT_MEAN, GNN_WEIGHT_GCN, GNN_WEIGHT_EDGE = 0, 1, 2, 3
 
 _lib = None
 _lock = threading.Lock()
@@ -82,6 +84,12 @@ PROTOTYPES: dict[str, tuple[object, list[object]]] = {
     "gnn_linear_int8_workspace_bytes": (_sz, [_vp, _i32, _i64, _vp, _i64, _i32, _i64, _i64, _i64]),
     "gnn_linear_int8_forward": (
         _i32, [_vp, _i32, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _sz, _vp]),
+    "gnn_spmm_int8_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "gnn_spmm_int8_forward": (
+        _i32, [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "gnn_group_norm_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "gnn_group_norm_forward": (
+        _i32, [_vp, _vp, _i32, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _i32, _vp, _sz, _vp]),
     "gnn_managed_alloc": (_i32, [_sz, _i32, ctypes.POINTER(_vp)]),
     "gnn_managed_free": (_i32, [_vp, _i32]),
     "gnn_hmm_supported": (_i32, [_i32, ctypes.POINTER(_i32)]),

@@ -319,6 +319,54 @@ int gnn_linear_int8_forward(const void* x, int x_type, int64_t ldx, const float*
                             int64_t ldo, float* out_scale, int64_t m, int64_t k, int64_t n, int relu,
                             void* workspace, size_t workspace_bytes, gnn_stream_t stream);
 
+/* How gnn_spmm_int8_forward weighs a neighbour's row. */
+typedef enum gnn_weighting {
+  GNN_WEIGHT_SUM = 0,  /* sum of rows                                     */
+  GNN_WEIGHT_MEAN = 1, /* sum / degree; 0 for a row without neighbours     */
+  GNN_WEIGHT_GCN = 2,  /* deg_inv_sqrt[r] * deg_inv_sqrt[c]                */
+  GNN_WEIGHT_EDGE = 3  /* edge_weight[e]                                   */
+} gnn_weighting;
+
+/* The aggregations of gnn_spmm_*_forward over 8-bit rows: out[r, :] (fp32, [num_nodes,
+ * feat_dim], contiguous) = f_r * sum_e w_e * x_scale[c] * x[c, :] in fp32. x is
+ * [num_nodes, feat_dim] with row stride ldx; deg_inv_sqrt / edge_weight as the
+ * weighting needs, else NULL. Deterministic, no atomics; the order of a row's sum
+ * differs from the fp32 entry points. Where x's base and ldx are multiples of 16 its
+ * rows are read in whole 16-byte pieces, so every row but the last must be backed by
+ * its full stride. Calls in flight at once need workspaces of their own
+ * (gnn_spmm_int8_workspace_bytes on the same device, 256-byte aligned). */
+size_t gnn_spmm_int8_workspace_bytes(int64_t num_nodes, int64_t num_edges, int64_t feat_dim);
+int gnn_spmm_int8_forward(const void* row_ptr, int row_ptr_type, const int32_t* col_ind, int weighting,
+                          const float* deg_inv_sqrt, const float* edge_weight, const int8_t* x, int64_t ldx,
+                          const float* x_scale, float* out, int64_t num_nodes, int64_t num_edges,
+                          int64_t feat_dim, void* workspace, size_t workspace_bytes, gnn_stream_t stream);
+
+/* ---- normalisation between layers -------------------------------------------- */
+
+typedef enum gnn_activation {
+  GNN_ACT_NONE = 0,
+  GNN_ACT_RELU = 1, /* max(y, 0) keeping -0 and NaN */
+  GNN_ACT_SILU = 2, /* y / (1 + exp(-y))            */
+  GNN_ACT_GELU = 3  /* y * (1 + erf(y / sqrt 2)) / 2 */
+} gnn_activation;
+
+/* Group normalisation with an activation over fp32 node features [num_nodes, channels]
+ * (no counterpart in the reference):
+ *   out = act((x - mean) / sqrt(var + eps) * weight[c] + bias[c])
+ * mean and biased variance over the channels / groups consecutive channels of a group,
+ * graph_ptr NULL: of each node on its own; else: of all nodes of a graph, graph g
+ * holding nodes [graph_ptr[g], graph_ptr[g + 1]) (num_graphs + 1 ascending offsets;
+ * offsets past num_nodes are taken as num_nodes). Rows of no graph are neither read
+ * nor written. groups = 1 normalises whole rows / graphs, groups = channels each
+ * channel. At most 1024 channels per group. weight and bias may be NULL. out may be
+ * x itself, else must not overlap it. Workspace: gnn_group_norm_workspace_bytes, with
+ * graph_ptr only. Deterministic, no atomics. */
+size_t gnn_group_norm_workspace_bytes(int64_t num_nodes, int64_t num_graphs, int64_t groups);
+int gnn_group_norm_forward(const float* x, const void* graph_ptr, int graph_ptr_type, int64_t num_graphs,
+                           const float* weight, const float* bias, float* out, int64_t num_nodes,
+                           int64_t channels, int64_t groups, float eps, int activation, void* workspace,
+                           size_t workspace_bytes, gnn_stream_t stream);
+
 /* ---- one layer in one pass: aggregation + dense transform ------------------- */
 
 /* Aggregations for gnn_fused_aggregate_linear. */

@@ -52,3 +52,23 @@ def test_python_refusals():
     t = I.empty_rows(5, 21, "cpu")
     assert t.shape == (5, 21) and t.stride(0) == 32
     assert I._overlap(t, t[2:]) and not I._overlap(t[:2], t[3:])
+
+
+def test_spmm_c_refusals():
+    L = N.lib()
+    p = 1 << 20
+    call = lambda n=4, e=4, f=8, ty=0, wt=0, dis=None, ew=None, x=p, ldx=8, ws=None, wsb=0: L.gnn_spmm_int8_forward(  # noqa: E731
+        p, ty, p, wt, dis, ew, x, ldx, p, p, n, e, f, ws, wsb, None)
+    assert call(n=-1) == 1 and call(ty=4) == 1 and call(wt=4) == 1 and call(wt=-1) == 1
+    assert call(e=1 << 31) == 1 and "int64 row_ptr" in N.last_error()
+    assert call(ldx=7) == 1
+    assert call(wt=2) == 2 and call(wt=3) == 2 and call(x=None) == 2
+    assert call() == 7 and "workspace" in N.last_error()
+    assert call(n=0) == 0 and call(f=0) == 0
+    assert L.gnn_spmm_int8_workspace_bytes(1000, 5000, 128) > 0
+
+
+def test_spmm_python_refusals():
+    rp, ci = torch.zeros(5, dtype=torch.int32), torch.zeros(0, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="out must be CUDA"):
+        I.spmm_int8_forward_(rp, ci, torch.zeros(4, 8, dtype=torch.int8), torch.ones(4), torch.zeros(4, 8))
