@@ -3,16 +3,14 @@
 // with (f_r, w_e) = (dis[r], dis[c_e]) for GCN, (1, edge_weight[e]) weighted,
 // (1, 1) sum and (1 / deg r, 1) mean; sums in fp32.
 //
-// Split: the merged sequence of row ends and entries is cut into equal shares, one
-// per warp (the cut points are found by a binary search on row_ptr), so hubs, short
-// and empty rows all balance. A warp stores the rows that lie wholly in its share;
-// what it holds of a row that began earlier, or ends later, goes to a workspace
-// slot, and a second small kernel adds those pieces in share order: no float
-// atomics, the same bits every time.
-//
-// Inside a warp a row takes L lanes of 16 columns each (one 128-bit load a lane), so
-// 32 / L entries are in flight per load; their sums are joined by a
-// reduce-scatter over the lane groups when the row ends.
+// Split: the merged sequence of row ends and entries is cut into equal shares (the
+// cut points are found by a binary search on row_ptr), so hubs, short and empty rows
+// all balance. A share is summed by a group of L lanes, 16 columns a lane: a warp
+// works on 32 / L shares at once, each load instruction brings 32 / L feature rows,
+// and nothing is joined across lanes. A group stores the rows that lie wholly in its
+// share; what it holds of a row that began earlier, or ends later, goes to a
+// workspace slot, and a second small kernel adds those pieces in share order: no
+// float atomics, the same bits every time.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -33,7 +31,8 @@ enum Mode : int { kSum = GNN_WEIGHT_SUM, kMean = GNN_WEIGHT_MEAN, kGcn = GNN_WEI
 struct I8SpmmArgs {
   const void* row_ptr;
   const int32_t* col;
-  const float* dis;
+  const float* dis;      // GCN row factors
+  const float* dis_col;  // GCN column factors; NULL where `scale` has them in already
   const float* ew;
   const int8_t* x;
   int64_t ldx;
@@ -41,35 +40,71 @@ struct I8SpmmArgs {
   float* out;
   int64_t n, nnz;
   int f;
-  int64_t share;    // row ends + entries per warp
+  int mode;
+  int64_t share;    // row ends + entries per lane group
   int64_t shares;   // number of shares
   float* part;      // [2 * shares, f]: head (row began earlier), tail (row ends later)
   int64_t* part_row;  // [shares] row of the tail piece, -1 none
 };
 
-// Four packed signed bytes as floats: each byte becomes the low mantissa bits of
-// 2^23 + 128 + q, from which 2^23 + 128 is taken off again (exact, no conversion unit).
-__device__ __forceinline__ void bytes_to_float(uint32_t v, float (&f)[4]) {
-  v ^= 0x80808080u;
-  constexpr float kBase = 8388736.0f;  // 2^23 + 128
-  f[0] = __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7540)) - kBase;
-  f[1] = __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7541)) - kBase;
-  f[2] = __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7542)) - kBase;
-  f[3] = __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7543)) - kBase;
-}
+// How feature rows can be read.
+enum Kind : int {
+  kWhole = 0,   // 16-byte aligned rows, f % 16 == 0
+  kRagged = 1,  // 16-byte aligned rows; the last lane's load runs past f within the stride
+  kBytes = 2    // any base and stride
+};
 
-// 16 bytes of row data starting at column c of a row of `f` columns.
-// VEC: rows start on 16-byte boundaries and the load may run past f within the
-// row's stride; `edge` marks the matrix's last row, whose stride may not be there.
-template <bool VEC>
-__device__ __forceinline__ uint4 load16(const int8_t* row, int c, int f, bool edge) {
-  if (VEC && (!edge || c + 16 <= f)) return __ldg(reinterpret_cast<const uint4*>(row + c));
+// 16 columns of row c; xl: the matrix's base plus this lane's first column c0. The
+// last row of the matrix may lack the storage behind its last column.
+template <int KIND>
+__device__ __forceinline__ uint4 load_row(const int8_t* xl, uint32_t ldx, int c, int c0, int f, int last_row) {
+  const int8_t* p = xl + static_cast<uint64_t>(static_cast<uint32_t>(c)) * ldx;
+  if (KIND == kWhole || (KIND == kRagged && (c0 + 16 <= f || c != last_row))) {
+    return __ldg(reinterpret_cast<const uint4*>(p));
+  }
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    if (c + i < f) w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(row + c + i))) << (8 * (i & 3));
+    if (c0 + i < f) w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(p + i))) << (8 * (i & 3));
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// acc += w * the four signed bytes of v, two columns an instruction. Each byte
+// becomes the low mantissa bits of 2^23 + 128 + q, from which 2^23 + 128 is taken off
+// again: exact, and without the conversion unit.
+__device__ __forceinline__ void fma_word(uint64_t ww, uint32_t v, uint64_t& a01, uint64_t& a23) {
+  v ^= 0x80808080u;
+  const uint32_t b0 = __byte_perm(v, 0x4b000000u, 0x7540), b1 = __byte_perm(v, 0x4b000000u, 0x7541);
+  const uint32_t b2 = __byte_perm(v, 0x4b000000u, 0x7542), b3 = __byte_perm(v, 0x4b000000u, 0x7543);
+  asm("{\n\t.reg .b64 p, q, m;\n\t"
+      "mov.b64 p, {%2, %3};\n\t"
+      "mov.b64 q, {%4, %5};\n\t"
+      "mov.b64 m, {%7, %7};\n\t"
+      "add.rn.f32x2 p, p, m;\n\t"
+      "add.rn.f32x2 q, q, m;\n\t"
+      "fma.rn.f32x2 %0, %6, p, %0;\n\t"
+      "fma.rn.f32x2 %1, %6, q, %1;\n\t}"
+      : "+l"(a01), "+l"(a23)
+      : "r"(b0), "r"(b1), "r"(b2), "r"(b3), "l"(ww), "r"(0xcb000080u));  // -(2^23 + 128)
+}
+
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+
+// eight floats, one 32-byte sector, not to be kept in the caches
+__device__ __forceinline__ void store8(float* p, const float* f) {
+  asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(__float_as_uint(f[0])),
+               "r"(__float_as_uint(f[1])), "r"(__float_as_uint(f[2])), "r"(__float_as_uint(f[3])),
+               "r"(__float_as_uint(f[4])), "r"(__float_as_uint(f[5])), "r"(__float_as_uint(f[6])),
+               "r"(__float_as_uint(f[7]))
+               : "memory");
 }
 
 template <class IdxT>
@@ -93,134 +128,139 @@ __device__ __forceinline__ int64_t row_at(const I8SpmmArgs& a, int64_t d) {
   return lo;
 }
 
-template <int MODE, class IdxT>
+template <class IdxT>
 __device__ __forceinline__ float row_factor(const I8SpmmArgs& a, int64_t r) {
-  if constexpr (MODE == kGcn) {
-    return __ldg(a.dis + r);
-  } else if constexpr (MODE == kMean) {
+  if (a.mode == kGcn) return __ldg(a.dis + r);
+  if (a.mode == kMean) {
     const int64_t deg = rp<IdxT>(a, r + 1) - rp<IdxT>(a, r);
     return deg > 0 ? __fdiv_rn(1.0f, static_cast<float>(deg)) : 0.0f;
-  } else {
-    return 1.0f;
   }
+  return 1.0f;
 }
 
-// L lanes per row (a power of two), 32 / L entries at a time.
-template <int MODE, int L, bool VEC, class IdxT>
-__global__ void __launch_bounds__(kThreads) spmm_i8_kernel(I8SpmmArgs a) {
-  constexpr int G = 32 / L;                    // lane groups
-  constexpr int KEEP = G >= 16 ? 1 : 16 / G;   // columns a lane holds after the reduce-scatter
-  const int lane = threadIdx.x & 31;
-  const int grp = lane / L;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (w >= a.shares) return;
-  const int cbase = blockIdx.y * kTileCols;    // L == 32 where f > 512, else 0
-  const int c0 = cbase + (lane % L) * 16;      // this lane's 16 columns
-  const bool have = c0 < a.f;
-  const int64_t total = a.n + a.nnz;
-  const int64_t d0 = w * a.share, d1 = min(d0 + a.share, total);
-  int64_t row = row_at<IdxT>(a, d0);
-  const int64_t row_end = row_at<IdxT>(a, d1);  // rows [row, row_end) end in this share
-  int64_t e = d0 - row;
-  const int64_t e_end = d1 - row_end;
-  bool head = row < a.n && rp<IdxT>(a, row) < e;  // the first row began in an earlier share
-  // column of the matrix that this lane keeps after the reduce-scatter
-  int keep_col = c0;
-#pragma unroll
-  for (int o = 16, half = 8; o >= L && half >= 1; o >>= 1, half >>= 1) keep_col += (lane & o) ? half : 0;
+// The weight of an entry whose column is c.
+__device__ __forceinline__ float entry_weight(const I8SpmmArgs& a, int c, int64_t e) {
+  float w = __ldg(a.scale + c);
+  if (a.dis_col != nullptr) w = __fmul_rn(w, __ldg(a.dis_col + c));
+  if (a.ew != nullptr) w = __fmul_rn(w, ld_stream_f32(a.ew + e));
+  return w;
+}
 
-  while (row < row_end || e < e_end) {
-    const bool ends = row < row_end;
-    const int64_t stop = ends ? rp<IdxT>(a, row + 1) : e_end;
-    float acc[16];
+// L lanes (4, 8, 16 or 32) per share. Entries are taken in chunks of L, one per
+// lane, whatever rows they belong to; the next chunk's weights and the columns of the
+// one after it are on their way while a chunk is summed, U feature rows in flight.
+template <int L, int KIND, class IdxT>
+__global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
+  constexpr int U = 2;
+  const int sub = threadIdx.x & (L - 1);
+  const int64_t w = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / L;  // share
+  // this lane's 16 columns; a lane past the last one reads the first ones and stores nothing
+  const int c0 = blockIdx.y * kTileCols + sub * 16;  // f > 512: column tiles
+  const bool have = c0 < a.f;
+  const int cl = have ? c0 : 0;
+  const int8_t* const xl = a.x + cl;
+  const uint32_t ldx = static_cast<uint32_t>(a.ldx);
+  const int last_row = static_cast<int>(a.n - 1);
+  // a group past the last share takes an empty one
+  const int64_t total = a.n + a.nnz;
+  const int64_t d0 = min(w * a.share, total), d1 = min(d0 + a.share, total);
+  int row = static_cast<int>(row_at<IdxT>(a, d0));
+  const int row_end = static_cast<int>(row_at<IdxT>(a, d1));  // rows [row, row_end) end in this share
+  const int64_t e0 = d0 - row;
+  const int len = static_cast<int>(d1 - row_end - e0);  // entries; positions are relative to e0
+  bool head = row < a.n && rp<IdxT>(a, row) < e0;       // the first row began in an earlier share
+  const bool open = e0 + len > max(e0, rp<IdxT>(a, row_end));  // the last entries' row ends in a later share
+  if (sub == 0 && blockIdx.y == 0 && w < a.shares) {
+    // the row that this share begins but does not end: its piece is the tail slot
+    a.part_row[w] = open && !(head && row == row_end) ? row_end : -1;
+  }
+  const int32_t* const cp = a.col + e0 + sub;
+  auto load_col = [&](int p) -> int { return p + sub < len ? ld_stream_i32(cp + p) : 0; };
+  // past the share: weight 0 on row 0
+  auto load_weight = [&](int p, int c) -> float {
+    return p + sub < len ? entry_weight(a, c, e0 + p + sub) : 0.0f;
+  };
+  auto load_stop = [&](int r) -> int {
+    return r < row_end ? static_cast<int>(rp<IdxT>(a, r + 1) - e0) : 0x7fffffff;
+  };
+  auto load_factor = [&](int r) -> float { return r < row_end ? row_factor<IdxT>(a, r) : 0.0f; };
+  float* const partl = a.part + 2 * w * a.f + c0;
+  const bool vec = (a.f & 7) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
+  uint64_t acc[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-    for (; e < stop; e += 32) {
-      const int cnt = static_cast<int>(min(static_cast<int64_t>(32), stop - e));
-      int c = 0;
-      float wt = 0.0f;
-      if (lane < cnt) {
-        c = ld_stream_i32(a.col + e + lane);
-        wt = __ldg(a.scale + c);
-        if constexpr (MODE == kGcn) wt = __fmul_rn(wt, __ldg(a.dis + c));
-        if constexpr (MODE == kWeighted) wt = __fmul_rn(wt, ld_stream_f32(a.ew + e + lane));
-      }
-      for (int j = 0; j < cnt; j += G) {
-        const int src = j + grp;
-        const int cj = __shfl_sync(kFull, c, src & 31);
-        const float wj = __shfl_sync(kFull, wt, src & 31);
-        if (src < cnt && have) {
-          const uint4 v = load16<VEC>(a.x + static_cast<int64_t>(cj) * a.ldx, c0, a.f, cj == a.n - 1);
-          const uint32_t b[4] = {v.x, v.y, v.z, v.w};
+  for (int i = 0; i < 8; ++i) acc[i] = 0;
+  // stores what was summed and starts anew
+  auto store = [&](float* dst, float fr) {
+    float f[16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float f4[4];
-            bytes_to_float(b[i], f4);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc[4 * i + k] = __fmaf_rn(wj, f4[k], acc[4 * i + k]);
-          }
-        }
-      }
+    for (int i = 0; i < 8; ++i) {
+      unpair(acc[i], f[2 * i], f[2 * i + 1]);
+      acc[i] = 0;
     }
-    e = stop;
-    // reduce-scatter over the lane groups: halves of the columns are exchanged until a
-    // lane holds KEEP of them; past 16 groups the last sums are taken whole
-    int width = 16;
 #pragma unroll
-    for (int o = 16; o >= L; o >>= 1) {
-      if (width > 1) {
-        const int half = width / 2;
-        const bool up = (lane & o) != 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (i < half) {
-            const float give = up ? acc[i] : acc[i + half];
-            const float keep = up ? acc[i + half] : acc[i];
-            acc[i] = keep + __shfl_xor_sync(kFull, give, o);
-          }
-        }
-        width = half;
-      } else {
-        acc[0] += __shfl_xor_sync(kFull, acc[0], o);
-      }
-    }
-    const bool whole = ends && !head;
-    float* dst;
-    if (whole) {
-      const float fr = row_factor<MODE, IdxT>(a, row);
-#pragma unroll
-      for (int i = 0; i < KEEP; ++i) acc[i] = __fmul_rn(acc[i], fr);
-      dst = a.out + row * a.f;
-    } else {
-      dst = a.part + (head ? 2 * w : 2 * w + 1) * a.f;
-    }
-    if (keep_col < a.f) {
-      if (KEEP >= 4 && keep_col + KEEP <= a.f && (a.f & 3) == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-#pragma unroll
-        for (int i = 0; i + 3 < KEEP; i += 4) {
-          *reinterpret_cast<float4*>(dst + keep_col + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-        }
+    for (int i = 0; i < 16; ++i) f[i] = __fmul_rn(f[i], fr);
+    if (have) {
+      if (vec) {
+        store8(dst, f);
+        if (c0 + 8 < a.f) store8(dst + 8, f + 8);
       } else {
 #pragma unroll
-        for (int i = 0; i < KEEP; ++i) {
-          if (keep_col + i < a.f) dst[keep_col + i] = acc[i];
+        for (int i = 0; i < 16; ++i) {
+          if (c0 + i < a.f) __stcs(dst + i, f[i]);
         }
       }
     }
-    if (!ends) break;
+  };
+  // where the current row and the next one end, and their factors
+  int stop = load_stop(row), stop_nxt = load_stop(row + 1);
+  float factor = load_factor(row), factor_nxt = load_factor(row + 1);
+  auto finish_row = [&]() {
+    // the row's sums, or the piece of a row that began earlier
+    store(head ? partl : a.out + static_cast<int64_t>(row) * a.f + c0, head ? 1.0f : factor);
     head = false;
     ++row;
+    stop = stop_nxt;
+    factor = factor_nxt;
+    stop_nxt = load_stop(row + 1);
+    factor_nxt = load_factor(row + 1);
+  };
+
+  int c_cur = load_col(0);
+  float w_cur = load_weight(0, c_cur);
+  int c_nxt = load_col(L);
+  for (int base = 0; __any_sync(kFull, base < len); base += L) {
+    const float w_nxt = load_weight(base + L, c_nxt);
+    const int c_far = load_col(base + 2 * L);
+#pragma unroll
+    for (int j = 0; j < L; j += U) {
+      if (L > 8 && !__any_sync(kFull, base + j < len)) break;
+      uint4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        v[u] = load_row<KIND>(xl, ldx, __shfl_sync(kFull, c_cur, j + u, L), cl, a.f, last_row);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float wt = __shfl_sync(kFull, w_cur, j + u, L);
+        while (stop == base + j + u && row < row_end) finish_row();
+        const uint64_t ww = pair(wt, wt);
+        fma_word(ww, v[u].x, acc[0], acc[1]);
+        fma_word(ww, v[u].y, acc[2], acc[3]);
+        fma_word(ww, v[u].z, acc[4], acc[5]);
+        fma_word(ww, v[u].w, acc[6], acc[7]);
+      }
+    }
+    c_cur = c_nxt;
+    w_cur = w_nxt;
+    c_nxt = c_far;
   }
-  // the row that this share began but did not end (its piece is the tail slot), if any
-  if (lane == 0 && blockIdx.y == 0) {
-    const bool tail = row_end < a.n && rp<IdxT>(a, row_end) < e_end && rp<IdxT>(a, row_end) + row_end >= d0;
-    a.part_row[w] = tail ? row_end : -1;
-  }
+  while (row < row_end) finish_row();               // rows that end with the share's last entry
+  if (open) store(head ? partl : partl + a.f, 1.0f);  // entries of a row that ends in a later share
 }
 
 // One warp per share whose tail piece begins a row: adds the head pieces of the
 // following shares up to the row's end.
-template <int MODE, class IdxT>
+template <class IdxT>
 __global__ void __launch_bounds__(kThreads) spmm_i8_join_kernel(I8SpmmArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
@@ -229,7 +269,7 @@ __global__ void __launch_bounds__(kThreads) spmm_i8_join_kernel(I8SpmmArgs a) {
   if (row < 0) return;
   // the row's end is item row_ptr[row + 1] + row of the merged sequence
   const int64_t last = (rp<IdxT>(a, row + 1) + row) / a.share;
-  const float fr = row_factor<MODE, IdxT>(a, row);
+  const float fr = row_factor<IdxT>(a, row);
   for (int c = lane; c < a.f; c += 32) {
     float s = a.part[(2 * w + 1) * a.f + c];
     for (int64_t k = w + 1; k <= last; ++k) s += a.part[2 * k * a.f + c];
@@ -237,63 +277,61 @@ __global__ void __launch_bounds__(kThreads) spmm_i8_join_kernel(I8SpmmArgs a) {
   }
 }
 
+__global__ void __launch_bounds__(kThreads) scale_table_kernel(const float* __restrict__ scale,
+                                                               const float* __restrict__ dis,
+                                                               float* __restrict__ table, int64_t n) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (i < n) table[i] = __fmul_rn(scale[i], dis[i]);
+}
+
+// GCN: scale[c] * dis[c] is tabulated first where the entries are many, which saves
+// one random 32-byte sector per entry; below, the extra launch costs more.
+bool use_table(int weighting, int64_t nnz) { return weighting == kGcn && nnz >= (int64_t(1) << 20); }
+
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
-// Items (row ends and entries) per warp: about 8 shares for each warp slot of the
-// device, at least 64 so that a share's pieces do not outweigh its rows.
-int64_t share_for(int64_t n, int64_t nnz) {
-  const int64_t slots = static_cast<int64_t>(sm_count()) * 48 * 4;
-  return std::max<int64_t>(64, std::min<int64_t>(2048, (n + nnz + slots - 1) / slots));
+int lanes_for(int64_t f) { return f <= 64 ? 4 : (f <= 128 ? 8 : (f <= 256 ? 16 : 32)); }
+
+// Items (row ends and entries) per share: about two shares for each lane group that
+// the device holds at once, at least 32 so that a share's pieces do not outweigh its rows.
+int64_t share_for(int64_t n, int64_t nnz, int64_t f) {
+  const int64_t groups = static_cast<int64_t>(sm_count()) * (1024 / lanes_for(f)) * 2;
+  return std::max<int64_t>(32, std::min<int64_t>(4096, (n + nnz + groups - 1) / groups));
 }
 
+// [tail rows][pieces][table]
 size_t workspace_for(int64_t n, int64_t nnz, int64_t f) {
-  const int64_t share = share_for(n, nnz);
+  const int64_t share = share_for(n, nnz, f);
   const int64_t shares = (n + nnz + share - 1) / share;
-  return static_cast<size_t>(round_up(shares * 8, 256) + round_up(2 * shares * f * 4, 256));
+  return static_cast<size_t>(round_up(shares * 8, 256) + round_up(2 * shares * f * 4, 256) +
+                             (use_table(kGcn, nnz) ? round_up(n * 4, 256) : 0));
 }
 
-template <int MODE, bool VEC, class IdxT>
-void launch_lanes(const I8SpmmArgs& a, cudaStream_t s) {
-  const unsigned blocks = static_cast<unsigned>((a.shares + kWarps - 1) / kWarps);
-  const unsigned tiles = static_cast<unsigned>((a.f + kTileCols - 1) / kTileCols);
-  const dim3 grid(blocks, tiles);
-  if (a.f <= 16) {
-    spmm_i8_kernel<MODE, 1, VEC, IdxT><<<grid, kThreads, 0, s>>>(a);
-  } else if (a.f <= 32) {
-    spmm_i8_kernel<MODE, 2, VEC, IdxT><<<grid, kThreads, 0, s>>>(a);
-  } else if (a.f <= 64) {
-    spmm_i8_kernel<MODE, 4, VEC, IdxT><<<grid, kThreads, 0, s>>>(a);
-  } else if (a.f <= 128) {
-    spmm_i8_kernel<MODE, 8, VEC, IdxT><<<grid, kThreads, 0, s>>>(a);
-  } else if (a.f <= 256) {
-    spmm_i8_kernel<MODE, 16, VEC, IdxT><<<grid, kThreads, 0, s>>>(a);
+template <int L, class IdxT>
+void launch(const I8SpmmArgs& a, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>((a.shares * L + kThreads - 1) / kThreads),
+                  static_cast<unsigned>((a.f + kTileCols - 1) / kTileCols));
+  if (((reinterpret_cast<uintptr_t>(a.x) | static_cast<uintptr_t>(a.ldx)) & 15) != 0) {
+    spmm_i8_kernel<L, kBytes, IdxT><<<grid, kThreads, 0, s>>>(a);
+  } else if (a.f % 16 != 0) {
+    spmm_i8_kernel<L, kRagged, IdxT><<<grid, kThreads, 0, s>>>(a);
   } else {
-    spmm_i8_kernel<MODE, 32, VEC, IdxT><<<grid, kThreads, 0, s>>>(a);
+    spmm_i8_kernel<L, kWhole, IdxT><<<grid, kThreads, 0, s>>>(a);
   }
-}
-
-template <int MODE, class IdxT>
-int run(const I8SpmmArgs& a, bool vec, cudaStream_t s) {
-  if (vec) {
-    launch_lanes<MODE, true, IdxT>(a, s);
-  } else {
-    launch_lanes<MODE, false, IdxT>(a, s);
-  }
-  GNN_LAUNCH_CHECK("spmm_i8_kernel launch");
-  spmm_i8_join_kernel<MODE, IdxT>
-      <<<static_cast<unsigned>((a.shares + kWarps - 1) / kWarps), kThreads, 0, s>>>(a);
-  GNN_LAUNCH_CHECK("spmm_i8_join_kernel launch");
-  return GNN_OK;
 }
 
 template <class IdxT>
-int run_mode(int mode, const I8SpmmArgs& a, bool vec, cudaStream_t s) {
-  switch (mode) {
-    case kSum: return run<kSum, IdxT>(a, vec, s);
-    case kMean: return run<kMean, IdxT>(a, vec, s);
-    case kGcn: return run<kGcn, IdxT>(a, vec, s);
-    default: return run<kWeighted, IdxT>(a, vec, s);
+int run(const I8SpmmArgs& a, cudaStream_t s) {
+  switch (lanes_for(a.f)) {
+    case 4: launch<4, IdxT>(a, s); break;
+    case 8: launch<8, IdxT>(a, s); break;
+    case 16: launch<16, IdxT>(a, s); break;
+    default: launch<32, IdxT>(a, s); break;
   }
+  GNN_LAUNCH_CHECK("spmm_i8_kernel launch");
+  spmm_i8_join_kernel<IdxT><<<static_cast<unsigned>((a.shares + kWarps - 1) / kWarps), kThreads, 0, s>>>(a);
+  GNN_LAUNCH_CHECK("spmm_i8_join_kernel launch");
+  return GNN_OK;
 }
 
 }  // namespace
@@ -324,6 +362,7 @@ extern "C" int gnn_spmm_int8_forward(const void* row_ptr, int row_ptr_type, cons
   }
   GNN_REQUIRE(num_nodes <= 0x7fffffffLL, GNN_ERR_UNSUPPORTED, "num_nodes must be <= 2^31 - 1");
   GNN_REQUIRE(feat_dim <= 65535LL * kTileCols, GNN_ERR_UNSUPPORTED, "feat_dim too large");
+  GNN_REQUIRE(ldx <= 0xffffffffLL, GNN_ERR_UNSUPPORTED, "row stride of x must be below 2^32");
   GNN_REQUIRE(ldx >= feat_dim, GNN_ERR_INVALID_ARGUMENT, "row stride of x must be >= feat_dim");
   GNN_REQUIRE(row_ptr != nullptr && out != nullptr, GNN_ERR_NULL_POINTER, "row_ptr and out must not be NULL");
   GNN_REQUIRE(num_edges == 0 || (col_ind != nullptr && x != nullptr && x_scale != nullptr), GNN_ERR_NULL_POINTER,
@@ -340,8 +379,10 @@ extern "C" int gnn_spmm_int8_forward(const void* row_ptr, int row_ptr_type, cons
   I8SpmmArgs a{};
   a.row_ptr = row_ptr;
   a.col = col_ind;
-  a.dis = deg_inv_sqrt;
-  a.ew = edge_weight;
+  a.mode = weighting;
+  a.dis = weighting == GNN_WEIGHT_GCN ? deg_inv_sqrt : nullptr;
+  a.dis_col = a.dis;
+  a.ew = weighting == GNN_WEIGHT_EDGE ? edge_weight : nullptr;
   a.x = x;
   a.ldx = ldx;
   a.scale = x_scale;
@@ -349,14 +390,20 @@ extern "C" int gnn_spmm_int8_forward(const void* row_ptr, int row_ptr_type, cons
   a.n = num_nodes;
   a.nnz = num_edges;
   a.f = static_cast<int>(feat_dim);
-  a.share = share_for(num_nodes, num_edges);
+  a.share = share_for(num_nodes, num_edges, feat_dim);
   a.shares = (num_nodes + num_edges + a.share - 1) / a.share;
   a.part_row = static_cast<int64_t*>(workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + round_up(a.shares * 8, 256));
-  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 16 == 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int rc = row_ptr_type == GNN_INDEX_INT32 ? run_mode<int32_t>(weighting, a, vec, s)
-                                                 : run_mode<int64_t>(weighting, a, vec, s);
+  if (use_table(weighting, num_edges)) {
+    float* table = a.part + round_up(2 * a.shares * feat_dim * 4, 256) / 4;
+    scale_table_kernel<<<static_cast<unsigned>((num_nodes + kThreads - 1) / kThreads), kThreads, 0, s>>>(
+        x_scale, deg_inv_sqrt, table, num_nodes);
+    GNN_LAUNCH_CHECK("scale_table_kernel launch");
+    a.scale = table;
+    a.dis_col = nullptr;
+  }
+  const int rc = row_ptr_type == GNN_INDEX_INT32 ? run<int32_t>(a, s) : run<int64_t>(a, s);
   if (rc == GNN_OK) clear_error();
   return rc;
 }
