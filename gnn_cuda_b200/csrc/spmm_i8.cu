@@ -151,7 +151,7 @@ __device__ __forceinline__ float entry_weight(const I8SpmmArgs& a, int c, int64_
 // one after it are on their way while a chunk is summed, U feature rows in flight.
 template <int L, int KIND, class IdxT>
 __global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
-  constexpr int U = 2;
+  constexpr int U = 4;
   const int sub = threadIdx.x & (L - 1);
   const int64_t w = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / L;  // share
   // this lane's 16 columns; a lane past the last one reads the first ones and stores nothing
@@ -258,23 +258,29 @@ __global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
   if (open) store(head ? partl : partl + a.f, 1.0f);  // entries of a row that ends in a later share
 }
 
-// One warp per share whose tail piece begins a row: adds the head pieces of the
-// following shares up to the row's end.
+// One warp per 32 columns of a share whose tail piece begins a row: adds the head
+// pieces of the following shares up to the row's end, eight loads in flight.
 template <class IdxT>
 __global__ void __launch_bounds__(kThreads) spmm_i8_join_kernel(I8SpmmArgs a) {
-  const int lane = threadIdx.x & 31;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   if (w >= a.shares) return;
   const int64_t row = a.part_row[w];
-  if (row < 0) return;
+  const int c = blockIdx.y * 32 + (threadIdx.x & 31);
+  if (row < 0 || c >= a.f) return;
   // the row's end is item row_ptr[row + 1] + row of the merged sequence
   const int64_t last = (rp<IdxT>(a, row + 1) + row) / a.share;
-  const float fr = row_factor<IdxT>(a, row);
-  for (int c = lane; c < a.f; c += 32) {
-    float s = a.part[(2 * w + 1) * a.f + c];
-    for (int64_t k = w + 1; k <= last; ++k) s += a.part[2 * k * a.f + c];
-    a.out[row * a.f + c] = __fmul_rn(s, fr);
+  const float* p = a.part + 2 * w * a.f + c;
+  float s = p[a.f];
+  int64_t k = w + 1;
+  for (; k + 8 <= last + 1; k += 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = a.part[2 * (k + i) * a.f + c];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += v[i];
   }
+  for (; k <= last; ++k) s += a.part[2 * k * a.f + c];
+  a.out[row * a.f + c] = __fmul_rn(s, row_factor<IdxT>(a, row));
 }
 
 __global__ void __launch_bounds__(kThreads) scale_table_kernel(const float* __restrict__ scale,
@@ -292,10 +298,10 @@ int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 int lanes_for(int64_t f) { return f <= 64 ? 4 : (f <= 128 ? 8 : (f <= 256 ? 16 : 32)); }
 
-// Items (row ends and entries) per share: about two shares for each lane group that
+// Items (row ends and entries) per share: about one share for each lane group that
 // the device holds at once, at least 32 so that a share's pieces do not outweigh its rows.
 int64_t share_for(int64_t n, int64_t nnz, int64_t f) {
-  const int64_t groups = static_cast<int64_t>(sm_count()) * (1024 / lanes_for(f)) * 2;
+  const int64_t groups = static_cast<int64_t>(sm_count()) * (1024 / lanes_for(f));
   return std::max<int64_t>(32, std::min<int64_t>(4096, (n + nnz + groups - 1) / groups));
 }
 
@@ -329,7 +335,8 @@ int run(const I8SpmmArgs& a, cudaStream_t s) {
     default: launch<32, IdxT>(a, s); break;
   }
   GNN_LAUNCH_CHECK("spmm_i8_kernel launch");
-  spmm_i8_join_kernel<IdxT><<<static_cast<unsigned>((a.shares + kWarps - 1) / kWarps), kThreads, 0, s>>>(a);
+  const dim3 grid(static_cast<unsigned>((a.shares + kWarps - 1) / kWarps), static_cast<unsigned>((a.f + 31) / 32));
+  spmm_i8_join_kernel<IdxT><<<grid, kThreads, 0, s>>>(a);
   GNN_LAUNCH_CHECK("spmm_i8_join_kernel launch");
   return GNN_OK;
 }
@@ -361,7 +368,7 @@ extern "C" int gnn_spmm_int8_forward(const void* row_ptr, int row_ptr_type, cons
     return GNN_OK;
   }
   GNN_REQUIRE(num_nodes <= 0x7fffffffLL, GNN_ERR_UNSUPPORTED, "num_nodes must be <= 2^31 - 1");
-  GNN_REQUIRE(feat_dim <= 65535LL * kTileCols, GNN_ERR_UNSUPPORTED, "feat_dim too large");
+  GNN_REQUIRE(feat_dim <= 65535LL * 32, GNN_ERR_UNSUPPORTED, "feat_dim too large");
   GNN_REQUIRE(ldx <= 0xffffffffLL, GNN_ERR_UNSUPPORTED, "row stride of x must be below 2^32");
   GNN_REQUIRE(ldx >= feat_dim, GNN_ERR_INVALID_ARGUMENT, "row stride of x must be >= feat_dim");
   GNN_REQUIRE(row_ptr != nullptr && out != nullptr, GNN_ERR_NULL_POINTER, "row_ptr and out must not be NULL");
