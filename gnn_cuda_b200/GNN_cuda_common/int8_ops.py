@@ -23,7 +23,7 @@ from __future__ import annotations
 import torch
 
 from .. import _native as N
-from .native_ops import _check, _index_type, _stream
+from .native_ops import _check, _index_type
 
 
 def empty_rows(rows: int, cols: int, device) -> torch.Tensor:
@@ -32,82 +32,123 @@ def empty_rows(rows: int, cols: int, device) -> torch.Tensor:
     return torch.empty(int(rows), (int(cols) + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :int(cols)]
 
 
-def _on_device(name: str, t: torch.Tensor, device: torch.device) -> None:
-    _check(t.is_cuda, f"{name} must be CUDA")
-    _check(t.device == device, f"{name} must be on the device of out")
+# The checks below are written for what they cost: small calls are bound by the host.
+# _current_stream and _current_device are torch.cuda.current_stream(d).cuda_stream and
+# torch.cuda.current_device() without the objects around them.
+_current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+_I8, _F32 = torch.int8, torch.float32
 
 
-def _check_rows8(name: str, t: torch.Tensor) -> None:
-    _check(t.dtype == torch.int8, f"{name} must be int8")
-    _check(t.dim() == 2, f"{name} must be rank-2")
-    _check(t.size(1) <= 1 or t.stride(1) == 1, f"{name} must have contiguous rows")
-    _check(t.size(0) <= 1 or t.stride(0) >= t.size(1), f"{name} must not have overlapping rows")
+def _device_of(out: torch.Tensor, name: str = "out") -> int:
+    """The output's device index; it is made current by _on() around the call."""
+    index = out.get_device()
+    _check(index >= 0 and out.is_cuda, f"{name} must be CUDA")
+    return index
 
 
-def _check_f32(name: str, t: torch.Tensor, dim: int, device: torch.device) -> None:
-    _on_device(name, t, device)
-    _check(t.dtype == torch.float32, f"{name} must be float32")
-    _check(t.dim() == dim, f"{name} must be rank-{dim}")
-    _check(t.is_contiguous(), f"{name} must be contiguous")
+def _same_device(name: str, t: torch.Tensor, index: int) -> None:
+    if t.get_device() != index or not t.is_cuda:
+        _check(t.is_cuda, f"{name} must be CUDA")
+        _check(False, f"{name} must be on the device of out")
 
 
-def _ld(t: torch.Tensor) -> int:
-    """Elements from row to row (a tensor of one row may report any stride)."""
-    return int(t.stride(0)) if t.size(0) > 1 else max(int(t.stride(0)), int(t.size(1)))
+def _check_rows8(name: str, t: torch.Tensor, index: int) -> int:
+    """Checks an int8 matrix of contiguous rows; returns the elements from row to row."""
+    _same_device(name, t, index)
+    if t.dtype is not _I8:
+        _check(False, f"{name} must be int8")
+    if t.dim() != 2:
+        _check(False, f"{name} must be rank-2")
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if cols > 1 and step != 1:
+        _check(False, f"{name} must have contiguous rows")
+    if rows > 1:
+        if ld < cols:
+            _check(False, f"{name} must not have overlapping rows")
+        return ld
+    return ld if ld > cols else cols  # a tensor of one row may report any stride
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the address ranges of two tensors of contiguous rows meet."""
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    end = lambda t: t.data_ptr() + ((t.size(0) - 1) * t.stride(0) + (t.size(1) if t.dim() > 1 else 1)) * t.element_size()  # noqa: E731
-    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+def _check_f32(name: str, t: torch.Tensor, dim: int, index: int) -> None:
+    _same_device(name, t, index)
+    if t.dtype is not _F32:
+        _check(False, f"{name} must be float32")
+    if t.dim() != dim:
+        _check(False, f"{name} must be rank-{dim}")
+    if not t.is_contiguous():
+        _check(False, f"{name} must be contiguous")
 
 
-class _Device:
-    """torch.cuda.device without its cost where the device is current already."""
+def _check_vector(name: str, t: torch.Tensor, length: int, index: int, what: str) -> None:
+    _check_f32(name, t, 1, index)
+    if t.shape[0] != length:
+        _check(False, f"{name} length must equal {what}")
 
-    def __init__(self, device: torch.device):
-        self.index = device.index
-        self.old = -1
+
+def _check_apart(out: torch.Tensor, out_ptr: int, out_ld: int, x: torch.Tensor, x_ptr: int, x_ld: int) -> None:
+    """Refuses an output whose address range meets that of x (matrices of contiguous rows)."""
+    if out_ptr <= x_ptr:
+        m, n = out.shape
+        first, last = x_ptr, out_ptr + ((m - 1) * out_ld + n) * out.element_size()
+    else:
+        m, n = x.shape
+        first, last = out_ptr, x_ptr + ((m - 1) * x_ld + n) * x.element_size()
+    if first < last and out.numel() and x.numel():
+        _check(False, "out must not alias x")
+
+
+class _On:
+    """torch.cuda.device(index), at the cost of one query where it is current already."""
+
+    __slots__ = ("index", "old")
+
+    def __init__(self, index: int):
+        self.index = index
 
     def __enter__(self):
-        now = torch.cuda.current_device()
+        now = _current_device() if _current_device else torch.cuda.current_device()
+        self.old = now
         if now != self.index:
-            self.old = now
             torch.cuda.set_device(self.index)
+        return _current_stream(self.index) if _current_stream else torch.cuda.current_stream(self.index).cuda_stream
 
     def __exit__(self, *exc):
-        if self.old >= 0:
+        if self.old != self.index:
             torch.cuda.set_device(self.old)
+
+
+def _scratch(nbytes: int, index: int) -> torch.Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index)) if nbytes else None
 
 
 def quantize_rows_(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
     """scale[i] = max|x[i]| / 127; q[i] = x[i] / scale[i] to the nearest integer, ties to
     even, on the exact quotient. Zero rows: scale 0, q 0. Rows with a NaN or an
     infinity: scale NaN, q 0 (what is computed from them is NaN)."""
-    _on_device("q", q, q.device)
-    _check_rows8("q", q)
-    _check_f32("x", x, 2, q.device)
-    _check_f32("scale", scale, 1, q.device)
-    _check(tuple(x.shape) == tuple(q.shape), "x and q must have the same shape")
-    _check(scale.numel() == x.size(0), "scale length must equal the number of rows")
-    with _Device(q.device):
-        N.call("gnn_quantize_rows", x.data_ptr(), x.size(1), x.size(0), x.size(1), q.data_ptr(), _ld(q),
-               scale.data_ptr(), _stream(q.device))
+    index = _device_of(q, "q")
+    ldq = _check_rows8("q", q, index)
+    _check_f32("x", x, 2, index)
+    rows, cols = x.shape
+    _check(x.shape == q.shape, "x and q must have the same shape")
+    _check_vector("scale", scale, rows, index, "the number of rows")
+    with _On(index) as stream:
+        N.check(N.lib().gnn_quantize_rows(x.data_ptr(), cols, rows, cols, q.data_ptr(), ldq, scale.data_ptr(), stream),
+                "gnn_quantize_rows")
 
 
 def quantize_weight_(weight: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
     """weight [in, out] (the layout of linear_forward_) as q [out, in] with one scale per output channel."""
-    _on_device("q", q, q.device)
-    _check_rows8("q", q)
-    _check_f32("weight", weight, 2, q.device)
-    _check_f32("scale", scale, 1, q.device)
-    _check(weight.size(0) == q.size(1) and weight.size(1) == q.size(0), "q must be [out, in] for weight [in, out]")
-    _check(scale.numel() == q.size(0), "scale length must equal the number of output channels")
-    with _Device(q.device):
-        N.call("gnn_quantize_weight", weight.data_ptr(), weight.size(0), weight.size(1), q.data_ptr(), _ld(q),
-               scale.data_ptr(), _stream(q.device))
+    index = _device_of(q, "q")
+    ldq = _check_rows8("q", q, index)
+    _check_f32("weight", weight, 2, index)
+    k, n = weight.shape
+    _check(k == q.shape[1] and n == q.shape[0], "q must be [out, in] for weight [in, out]")
+    _check_vector("scale", scale, n, index, "the number of output channels")
+    with _On(index) as stream:
+        N.check(N.lib().gnn_quantize_weight(weight.data_ptr(), k, n, q.data_ptr(), ldq, scale.data_ptr(), stream),
+                "gnn_quantize_weight")
 
 
 def linear_int8_forward_(x: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.Tensor,
@@ -119,55 +160,52 @@ def linear_int8_forward_(x: torch.Tensor, x_scale: torch.Tensor | None, weight: 
     quantised on the way). weight: int8 [n, k] with weight_scale [n]
     (``quantize_weight_``). out: float32 [m, n], or int8 [m, n] with out_scale [m]
     (quantised as ``quantize_rows_`` would quantise the float32 result)."""
-    dev = out.device
-    _check(out.is_cuda, "out must be CUDA")
-    _on_device("x", x, dev)
-    _on_device("weight", weight, dev)
-    _check_rows8("weight", weight)
-    _check_f32("weight_scale", weight_scale, 1, dev)
-    if x.dtype == torch.int8:
-        _check_rows8("x", x)
+    index = _device_of(out)
+    ldw = _check_rows8("weight", weight, index)
+    n, k = weight.shape
+    _check_vector("weight_scale", weight_scale, n, index, "the number of output channels")
+    if x.dtype is _I8:
+        ldx = _check_rows8("x", x, index)
         _check(x_scale is not None, "x_scale is needed for int8 x")
-        _check_f32("x_scale", x_scale, 1, dev)
-        _check(x_scale.numel() == x.size(0), "x_scale length must equal the number of rows")
-        x_type = N.GNN_ROWS_INT8
+        _check_vector("x_scale", x_scale, x.shape[0], index, "the number of rows")
+        x_type, xs_ptr = N.GNN_ROWS_INT8, x_scale.data_ptr()
     else:
-        _check(x.dtype == torch.float32, "x must be int8 or float32")
-        _check_f32("x", x, 2, dev)
+        _check(x.dtype is _F32, "x must be int8 or float32")
+        _check_f32("x", x, 2, index)
         _check(x_scale is None, "x_scale must be None for float32 x")
-        x_type = N.GNN_ROWS_FP32
-    m, k, n = x.size(0), x.size(1), weight.size(0)
-    _check(k == weight.size(1), "Inner GEMM dimensions must match")
+        x_type, xs_ptr, ldx = N.GNN_ROWS_FP32, None, x.shape[1]
+    m = x.shape[0]
+    _check(k == x.shape[1], "Inner GEMM dimensions must match")
     _check(k >= 1, "x must have at least one column")
-    _check(weight_scale.numel() == n, "weight_scale length must equal the number of output channels")
-    _check(out.dim() == 2 and out.size(0) == m and out.size(1) == n, "Output shape must match x @ weight")
-    if out.dtype == torch.int8:
-        _check_rows8("out", out)
+    _check(out.dim() == 2 and out.shape[0] == m and out.shape[1] == n, "Output shape must match x @ weight")
+    if out.dtype is _I8:
+        ldo = _check_rows8("out", out, index)
         _check(out_scale is not None, "out_scale is needed for int8 out")
-        _check_f32("out_scale", out_scale, 1, dev)
-        _check(out_scale.numel() == m, "out_scale length must equal the number of rows")
-        out_type = N.GNN_ROWS_INT8
+        _check_vector("out_scale", out_scale, m, index, "the number of rows")
+        out_type, os_ptr = N.GNN_ROWS_INT8, out_scale.data_ptr()
     else:
-        _check(out.dtype == torch.float32, "out must be int8 or float32")
+        _check(out.dtype is _F32, "out must be int8 or float32")
         _check(out.is_contiguous(), "out must be contiguous")
         _check(out_scale is None, "out_scale must be None for float32 out")
-        out_type = N.GNN_ROWS_FP32
+        out_type, os_ptr, ldo = N.GNN_ROWS_FP32, None, n
+    bias_ptr = None
     if bias is not None and bias.numel() != 0:
-        _check_f32("bias", bias, 1, dev)
-        _check(bias.numel() == n, "bias length must equal output feature dimension")
+        _check_vector("bias", bias, n, index, "output feature dimension")
         bias_ptr = bias.data_ptr()
-    else:
-        bias_ptr = None
-    _check(not _overlap(out, x), "out must not alias x")
-    L = N.lib()
-    xp, ldx, wp, ldw = x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight)
-    with _Device(dev):
-        wsb = L.gnn_linear_int8_workspace_bytes(xp, x_type, ldx, wp, ldw, out_type, m, k, n)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-        N.check(L.gnn_linear_int8_forward(
-            xp, x_type, ldx, None if x_scale is None else x_scale.data_ptr(), wp, ldw, weight_scale.data_ptr(), bias_ptr,
-            out.data_ptr(), out_type, _ld(out), None if out_scale is None else out_scale.data_ptr(), m, k, n,
-            1 if relu else 0, None if ws is None else ws.data_ptr(), wsb, _stream(dev)), "gnn_linear_int8_forward")
+    xp, wp, op = x.data_ptr(), weight.data_ptr(), out.data_ptr()
+    _check_apart(out, op, ldo, x, xp, ldx)
+    lib = N.lib()
+    args = (xp, x_type, ldx, xs_ptr, wp, ldw, weight_scale.data_ptr(), bias_ptr, op, out_type, ldo, os_ptr, m, k, n,
+            1 if relu else 0)
+    with _On(index) as stream:
+        # most calls need no scratch: the entry point says where one does, before it launches anything
+        rc = lib.gnn_linear_int8_forward(*args, None, 0, stream)
+        if rc == N.GNN_ERR_WORKSPACE:
+            wsb = lib.gnn_linear_int8_workspace_bytes(xp, x_type, ldx, wp, ldw, out_type, m, k, n)
+            ws = _scratch(wsb, index)
+            rc = lib.gnn_linear_int8_forward(*args, ws.data_ptr(), wsb, stream)
+        if rc:
+            N.check(rc, "gnn_linear_int8_forward")
 
 
 _WEIGHTING = {"sum": N.GNN_WEIGHT_SUM, "mean": N.GNN_WEIGHT_MEAN, "gcn": N.GNN_WEIGHT_GCN,
@@ -185,44 +223,42 @@ def spmm_int8_forward_(row_ptr: torch.Tensor, col_ind: torch.Tensor, x: torch.Te
     ``spmm_pyg_gcn_forward_``. x: int8 [num_nodes, f] with x_scale [num_nodes]; out:
     float32 [num_nodes, f]. Rows are summed in another order than the float32
     aggregations, the same one in every call."""
-    dev = out.device
-    _check(out.is_cuda, "out must be CUDA")
-    _check(aggregation in _WEIGHTING, "aggregation must be sum, mean, gcn or weighted")
-    for name, t in (("row_ptr", row_ptr), ("col_ind", col_ind), ("x", x)):
-        _on_device(name, t, dev)
+    index = _device_of(out)
+    weighting = _WEIGHTING.get(aggregation)
+    _check(weighting is not None, "aggregation must be sum, mean, gcn or weighted")
     for name, t in (("row_ptr", row_ptr), ("col_ind", col_ind)):
+        _same_device(name, t, index)
         _check(t.is_contiguous(), f"{name} must be contiguous")
         _check(t.dim() == 1, f"{name} must be rank-1")
-    _check(row_ptr.dtype in (torch.int32, torch.int64), "row_ptr must be int32")
-    _check(col_ind.dtype == torch.int32, "col_ind must be int32")
-    _check_rows8("x", x)
-    _check_f32("x_scale", x_scale, 1, dev)
-    _check_f32("out", out, 2, dev)
-    _check(tuple(x.shape) == tuple(out.shape), "x and out must have the same shape")
-    n, f, nnz = x.size(0), x.size(1), col_ind.numel()
-    _check(x_scale.numel() == n, "x_scale length must equal num_nodes")
-    _check(row_ptr.numel() == n + 1, "row_ptr length must be num_nodes + 1")
+    row_type = _index_type(row_ptr)
+    _check(col_ind.dtype is torch.int32, "col_ind must be int32")
+    ldx = _check_rows8("x", x, index)
+    _check_f32("out", out, 2, index)
+    _check(x.shape == out.shape, "x and out must have the same shape")
+    n, f = out.shape
+    nnz = col_ind.shape[0]
+    _check_vector("x_scale", x_scale, n, index, "num_nodes")
+    _check(row_ptr.shape[0] == n + 1, "row_ptr length must be num_nodes + 1")
     dis_ptr = ew_ptr = None
     if aggregation == "gcn":
         _check(deg_inv_sqrt is not None, "deg_inv_sqrt is needed for gcn")
-        _check_f32("deg_inv_sqrt", deg_inv_sqrt, 1, dev)
-        _check(deg_inv_sqrt.numel() == n, "deg_inv_sqrt length must equal num_nodes")
+        _check_vector("deg_inv_sqrt", deg_inv_sqrt, n, index, "num_nodes")
         dis_ptr = deg_inv_sqrt.data_ptr()
     else:
         _check(deg_inv_sqrt is None, "deg_inv_sqrt is only for gcn")
     if aggregation == "weighted":
         _check(edge_weight is not None, "edge_weight is needed for weighted")
-        _check_f32("edge_weight", edge_weight, 1, dev)
-        _check(edge_weight.numel() == nnz, "col_ind and edge_weight lengths must match")
+        _check_vector("edge_weight", edge_weight, nnz, index, "the number of entries")
         ew_ptr = edge_weight.data_ptr()
     else:
         _check(edge_weight is None, "edge_weight is only for weighted")
-    _check(not _overlap(out, x), "out must not alias x")
-    L = N.lib()
-    with _Device(dev):
-        wsb = L.gnn_spmm_int8_workspace_bytes(n, nnz, f)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-        N.check(L.gnn_spmm_int8_forward(
-            row_ptr.data_ptr(), _index_type(row_ptr), col_ind.data_ptr(), _WEIGHTING[aggregation], dis_ptr, ew_ptr,
-            x.data_ptr(), _ld(x), x_scale.data_ptr(), out.data_ptr(), n, nnz, f, ws.data_ptr(), wsb, _stream(dev)),
-            "gnn_spmm_int8_forward")
+    xp, op = x.data_ptr(), out.data_ptr()
+    _check_apart(out, op, f, x, xp, ldx)
+    lib = N.lib()
+    with _On(index) as stream:
+        wsb = lib.gnn_spmm_int8_workspace_bytes(n, nnz, f)
+        ws = _scratch(wsb, index)
+        N.check(lib.gnn_spmm_int8_forward(row_ptr.data_ptr(), row_type, col_ind.data_ptr(), weighting, dis_ptr, ew_ptr,
+                                          xp, ldx, x_scale.data_ptr(), op, n, nnz, f,
+                                          None if ws is None else ws.data_ptr(), wsb, stream),
+                "gnn_spmm_int8_forward")

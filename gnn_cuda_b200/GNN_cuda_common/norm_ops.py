@@ -12,8 +12,8 @@ from __future__ import annotations
 import torch
 
 from .. import _native as N
-from .int8_ops import _check_f32, _Device, _on_device, _overlap
-from .native_ops import _check, _index_type, _stream
+from .int8_ops import _check_apart, _check_f32, _check_vector, _device_of, _On, _same_device, _scratch
+from .native_ops import _check, _index_type
 
 ACTIVATIONS = {"none": N.GNN_ACT_NONE, "relu": N.GNN_ACT_RELU, "silu": N.GNN_ACT_SILU, "gelu": N.GNN_ACT_GELU}
 
@@ -26,32 +26,39 @@ def group_norm_forward_(x: torch.Tensor, groups: int, weight: torch.Tensor | Non
     graph_ptr: int32 or int64 [num_graphs + 1] ascending row offsets; rows before the
     first and behind the last are left as they are in out. activation: none, relu,
     silu or gelu (erf). weight / bias: [channels] or None. out may be x itself."""
-    dev = out.device
-    _check_f32("out", out, 2, dev)
-    _check_f32("x", x, 2, dev)
-    _check(tuple(x.shape) == tuple(out.shape), "x and out must have the same shape")
-    n, c = x.size(0), x.size(1)
+    index = _device_of(out)
+    _check_f32("out", out, 2, index)
+    _check_f32("x", x, 2, index)
+    _check(x.shape == out.shape, "x and out must have the same shape")
+    n, c = x.shape
     groups = int(groups)
     _check(groups >= 1 and c % groups == 0, "groups must be >= 1 and divide the number of channels")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _check_f32(name, t, 1, dev)
-            _check(t.numel() == c, f"{name} length must equal the number of channels")
-    _check(activation in ACTIVATIONS, "activation must be none, relu, silu or gelu")
-    _check(float(eps) >= 0.0, "eps must be >= 0")
-    _check(x.data_ptr() == out.data_ptr() or not _overlap(out, x), "out must be x itself or not overlap it")
+    w_ptr = b_ptr = None
+    if weight is not None:
+        _check_vector("weight", weight, c, index, "the number of channels")
+        w_ptr = weight.data_ptr()
+    if bias is not None:
+        _check_vector("bias", bias, c, index, "the number of channels")
+        b_ptr = bias.data_ptr()
+    act = ACTIVATIONS.get(activation)
+    _check(act is not None, "activation must be none, relu, silu or gelu")
+    eps = float(eps)
+    _check(eps >= 0.0, "eps must be >= 0")
+    xp, op = x.data_ptr(), out.data_ptr()
+    if xp != op:
+        _check_apart(out, op, c, x, xp, c)
     ptr, ptr_type, graphs = None, N.GNN_INDEX_INT32, 0
     if graph_ptr is not None:
-        _on_device("graph_ptr", graph_ptr, dev)
+        _same_device("graph_ptr", graph_ptr, index)
         _check(graph_ptr.dtype in (torch.int32, torch.int64), "graph_ptr must be int32 or int64")
         _check(graph_ptr.dim() == 1 and graph_ptr.is_contiguous(), "graph_ptr must be rank-1 and contiguous")
-        _check(graph_ptr.numel() >= 1, "graph_ptr must hold num_graphs + 1 offsets")
-        ptr, ptr_type, graphs = graph_ptr.data_ptr(), _index_type(graph_ptr), graph_ptr.numel() - 1
-    L = N.lib()
-    with _Device(dev):
-        wsb = L.gnn_group_norm_workspace_bytes(n, graphs, groups) if ptr is not None else 0
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-        N.check(L.gnn_group_norm_forward(
-            x.data_ptr(), ptr, ptr_type, graphs, None if weight is None else weight.data_ptr(),
-            None if bias is None else bias.data_ptr(), out.data_ptr(), n, c, groups, float(eps), ACTIVATIONS[activation],
-            None if ws is None else ws.data_ptr(), wsb, _stream(dev)), "gnn_group_norm_forward")
+        graphs = graph_ptr.shape[0] - 1
+        _check(graphs >= 0, "graph_ptr must hold num_graphs + 1 offsets")
+        ptr, ptr_type = graph_ptr.data_ptr(), _index_type(graph_ptr)
+    lib = N.lib()
+    with _On(index) as stream:
+        wsb = lib.gnn_group_norm_workspace_bytes(n, graphs, groups) if ptr is not None else 0
+        ws = _scratch(wsb, index)
+        N.check(lib.gnn_group_norm_forward(xp, ptr, ptr_type, graphs, w_ptr, b_ptr, op, n, c, groups, eps, act,
+                                           None if ws is None else ws.data_ptr(), wsb, stream),
+                "gnn_group_norm_forward")

@@ -17,6 +17,7 @@ LIB_PATH = Path(os.environ.get("GNNB200_LIB", _PKG / "libgnnb200.so"))
 
 GNN_OK = 0
 GNN_ERR_UNSUPPORTED = 3
+GNN_ERR_WORKSPACE = 7
 GNN_AGG_GCN, GNN_AGG_SUM, GNN_AGG_MEAN, GNN_AGG_MEAN_RECIPROCAL = 0, 1, 2, 3
 GNN_INDEX_INT32, GNN_INDEX_INT64 = 0, 1
 GNN_PRECISION_TF32, GNN_PRECISION_FP32 = 0, 1

@@ -400,6 +400,100 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps<BN, OUT8>(), 1)
   }
 }
 
+// ---- a few rows ----------------------------------------------------------------
+//
+// Up to kSmallRows rows are bound by latency and by reading w once, so no tensor core
+// is set up: one kernel quantises the rows (fp32 input; every block for itself, they
+// are small) into shared memory, zero-padded to 16 columns, and a warp takes an output
+// channel, 16 bytes of w a lane, with four-way 8-bit dot products.
+constexpr int kSmallRows = 8;
+constexpr int kSmallBytes = 40 * 1024;  // shared memory for the rows
+constexpr int kSmallThreads = 256;
+
+struct SmallParams {
+  const void* x;
+  int64_t ldx;
+  const float* x_scale;  // NULL: x is fp32
+  const int8_t* w;
+  int64_t ldw;
+  const float* w_scale;
+  const float* bias;
+  float* out;
+  int64_t ldo;
+  int m, k, n;
+  int relu;
+};
+
+template <int MR>
+__global__ void __launch_bounds__(kSmallThreads) linear_i8_small_kernel(SmallParams p) {
+  extern __shared__ __align__(16) int8_t sx[];  // [m][pitch]
+  __shared__ float sscale[kSmallRows];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunks = (p.k + 15) / 16;
+  const int pitch = chunks * 16;
+  int64_t j = static_cast<int64_t>(blockIdx.x) * (kSmallThreads / 32) + warp;
+  // 16 bytes of row j of w; its last piece byte by byte where the last row may end
+  auto load_w = [&](int64_t row, int c) -> uint4 {
+    const int8_t* src = p.w + row * p.ldw + c * 16;
+    if (c * 16 + 16 <= p.k || row < p.n - 1) return __ldg(reinterpret_cast<const uint4*>(src));
+    uint32_t v[4] = {0, 0, 0, 0};
+    for (int i = 0; c * 16 + i < p.k; ++i) {
+      v[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(src + i))) << (8 * (i & 3));
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  };
+  uint4 first = make_uint4(0, 0, 0, 0);  // on its way while the rows are quantised
+  if (j < p.n && lane < chunks) first = load_w(j, lane);
+
+  for (int r = warp; r < p.m; r += kSmallThreads / 32) {
+    int8_t* dst = sx + r * pitch;
+    if (p.x_scale == nullptr) {
+      const float* src = static_cast<const float*>(p.x) + r * p.ldx;
+      float amax = 0.0f;
+      for (int c = lane; c < p.k; c += 32) amax = max_abs_nan(amax, __ldg(src + c));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) amax = max_abs_nan(amax, __shfl_xor_sync(kFull, amax, o));
+      const RowQuant rq = row_quant(amax);
+      for (int c = lane; c < pitch; c += 32) dst[c] = c < p.k ? quant1(rq, __ldg(src + c)) : int8_t(0);
+      if (lane == 0) sscale[r] = rq.s;
+    } else {
+      const int8_t* src = static_cast<const int8_t*>(p.x) + r * p.ldx;
+      for (int c = lane; c < pitch; c += 32) dst[c] = c < p.k ? __ldg(src + c) : int8_t(0);
+      if (lane == 0) sscale[r] = __ldg(p.x_scale + r);
+    }
+  }
+  __syncthreads();
+
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kSmallThreads / 32);
+  for (bool again = false; j < p.n; j += step, again = true) {
+    int acc[MR];
+#pragma unroll
+    for (int r = 0; r < MR; ++r) acc[r] = 0;
+    for (int c = lane; c < chunks; c += 32) {
+      const uint4 w = (c == lane && !again) ? first : load_w(j, c);
+#pragma unroll
+      for (int r = 0; r < MR; ++r) {
+        if (r < p.m) {
+          const uint4 v = *reinterpret_cast<const uint4*>(sx + r * pitch + c * 16);
+          acc[r] = __dp4a(static_cast<int>(v.x), static_cast<int>(w.x), acc[r]);
+          acc[r] = __dp4a(static_cast<int>(v.y), static_cast<int>(w.y), acc[r]);
+          acc[r] = __dp4a(static_cast<int>(v.z), static_cast<int>(w.z), acc[r]);
+          acc[r] = __dp4a(static_cast<int>(v.w), static_cast<int>(w.w), acc[r]);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < MR; ++r) acc[r] = __reduce_add_sync(kFull, acc[r]);
+    if (lane < p.m) {
+      int mine = acc[0];
+#pragma unroll
+      for (int r = 1; r < MR; ++r) mine = lane == r ? acc[r] : mine;
+      p.out[lane * p.ldo + j] = scaled(mine, sscale[lane], __ldg(p.w_scale + j),
+                                       p.bias != nullptr ? __ldg(p.bias + j) : 0.0f, p.bias != nullptr, p.relu != 0);
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -480,6 +574,28 @@ int launch(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int64_t k
   return launch_bn<256, OUT8>(x, ldx, w, ldw, k, p, stream);
 }
 
+// Whether the few-rows kernel takes the call: fp32 output, aligned w, rows that fit.
+bool small_call(const int8_t* w, int64_t ldw, int out_type, int64_t m, int64_t k) {
+  return out_type == GNN_ROWS_FP32 && m <= kSmallRows && m * round_up(k, 16) <= kSmallBytes && aligned_rows(w, ldw);
+}
+
+int launch_small(const SmallParams& p, cudaStream_t stream) {
+  const size_t smem = static_cast<size_t>(p.m) * round_up(p.k, 16);
+  const unsigned grid = static_cast<unsigned>(
+      std::min<int64_t>((p.n + kSmallThreads / 32 - 1) / (kSmallThreads / 32), 8LL * sm_count()));
+  if (p.m <= 1) {
+    linear_i8_small_kernel<1><<<grid, kSmallThreads, smem, stream>>>(p);
+  } else if (p.m <= 2) {
+    linear_i8_small_kernel<2><<<grid, kSmallThreads, smem, stream>>>(p);
+  } else if (p.m <= 4) {
+    linear_i8_small_kernel<4><<<grid, kSmallThreads, smem, stream>>>(p);
+  } else {
+    linear_i8_small_kernel<8><<<grid, kSmallThreads, smem, stream>>>(p);
+  }
+  GNN_LAUNCH_CHECK("linear_i8_small_kernel launch");
+  return GNN_OK;
+}
+
 constexpr int64_t kMaxRow8 = 256;  // widest 8-bit output row that one tile holds
 
 // Workspace: [quantised or repacked x][its scales][repacked w][fp32 rows of a wide 8-bit output]
@@ -491,6 +607,7 @@ struct Plan {
 Plan plan_for(const void* x, int x_type, int64_t ldx, const int8_t* w, int64_t ldw, int out_type, int64_t m, int64_t k,
               int64_t n) {
   Plan p;
+  if (small_call(w, ldw, out_type, m, k)) return p;
   const int64_t pitch = round_up(std::max<int64_t>(k, 1), 16);
   if (x_type == GNN_ROWS_FP32) {
     p.x_bytes = round_up(m * pitch, 256);
@@ -554,6 +671,14 @@ extern "C" int gnn_linear_int8_forward(const void* x, int x_type, int64_t ldx, c
   GNN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, GNN_ERR_WORKSPACE,
               "workspace must be 256-byte aligned");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (small_call(weight, ldw, out_type, m, k)) {
+    const SmallParams sp{x, ldx, x_type == GNN_ROWS_FP32 ? nullptr : x_scale, weight, ldw, weight_scale, bias,
+                         static_cast<float*>(out), ldo, static_cast<int>(m), static_cast<int>(k), static_cast<int>(n),
+                         relu ? 1 : 0};
+    const int rc = launch_small(sp, s);
+    if (rc == GNN_OK) clear_error();
+    return rc;
+  }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int64_t pitch = round_up(k, 16);
   int rc = GNN_OK;

@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <mutex>
 
 namespace gnnb200 {
@@ -30,14 +31,19 @@ inline EncodeTiledFn encode_fn() {
 }
 
 inline bool device_is_sm100() {
+  static std::atomic<int> known[64] = {};  // per device: 0 not asked yet, 1 no, 2 yes
   int dev = 0, major = 0, minor = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
     return false;
   }
+  const bool slot = dev >= 0 && dev < 64;
+  if (slot && known[dev].load(std::memory_order_relaxed) != 0) return known[dev].load(std::memory_order_relaxed) == 2;
   cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
   cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
-  return major == 10 && minor == 0;
+  const bool yes = major == 10 && minor == 0;
+  if (slot) known[dev].store(yes ? 2 : 1, std::memory_order_relaxed);
+  return yes;
 }
 
 }  // namespace gnnb200

@@ -51,7 +51,20 @@ def test_python_refusals():
         I.linear_int8_forward_(x8, s, x8, s, None, torch.zeros(4, 4))
     t = I.empty_rows(5, 21, "cpu")
     assert t.shape == (5, 21) and t.stride(0) == 32
-    assert I._overlap(t, t[2:]) and not I._overlap(t[:2], t[3:])
+
+
+def test_overlap_check():
+    base = torch.empty(10, 32, dtype=torch.int8)
+
+    def apart(a, b):
+        I._check_apart(a, a.data_ptr(), a.stride(0), b, b.data_ptr(), b.stride(0))
+
+    apart(base[:2], base[3:])
+    apart(base[5:], base[:5, :7])
+    apart(base[:0], base)
+    for a, b in ((base, base[2:]), (base[2:], base), (base[3:6], base[5:])):
+        with pytest.raises(RuntimeError, match="must not alias"):
+            apart(a, b)
 
 
 def test_spmm_c_refusals():
