@@ -3,20 +3,22 @@
 // with mean and (biased) variance over the C / groups channels of a group, either
 // of each node on its own, or of all nodes of a graph of a batch (graph_ptr, ragged).
 //
-// Statistics: a warp reads rows in batches of U; each lane folds a batch's mean and
-// squared deviations about it into its running ones (the pairwise update of mean and
-// M2), so nothing is subtracted from a large sum; lanes, then pieces, are joined the
-// same way. The result is the same every time: no atomics.
+// Statistics: each lane folds a batch of rows' mean and squared deviations about it
+// into its running ones (the pairwise update of mean and M2), so nothing is
+// subtracted from a large sum; lanes, warps, then pieces, are joined the same way.
+// The result is the same every time: no floating-point atomics.
 //
-// Batch mode: rows are cut into chunks of kChunk, one warp each. A graph of at most
-// kChunk nodes belongs to the warp in whose chunk it starts and is finished there
-// (its second read comes from L1 / L2). A longer graph leaves a piece per chunk in
-// the workspace; a second kernel joins the pieces, a third reads x again and writes.
-// So a long graph costs three passes over its rows where x exceeds the L2.
+// Batch mode: rows are cut into windows, one block each. A graph of at most kShort
+// nodes belongs to the block in whose window it starts and is finished there, from
+// registers where its rows fit them (8 warps x U rows), else with a second read from
+// L1 / L2; so is a longer one that lies inside the window. Another graph leaves a piece per window in the workspace; a second kernel
+// joins the pieces, a third reads x again and writes. So a long graph costs three
+// passes over its rows where x exceeds the L2.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -24,9 +26,13 @@ namespace gnnb200 {
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kChunk = 64;        // rows per warp; the longest graph that one warp finishes
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kShort = 64;        // the longest graph that one block finishes
 constexpr int kTile = 1024;       // channels per column tile at most (whole groups)
-constexpr int kJoinThreads = 512;
+constexpr int kFewPieces = 64;    // pieces that one warp joins
+constexpr int kMaxWindow = 512;   // rows per block at most
+constexpr int kMaxLongs = kMaxWindow / kShort + 2;  // long graphs that meet a window
 
 struct NormArgs {
   const float* x;
@@ -34,62 +40,99 @@ struct NormArgs {
   const float* bias;
   float* out;
   const void* ptr;    // graph offsets, batch mode
+  int wide_ptr;       // they are int64
   int64_t graphs;
   int64_t n;
   int c, groups, cg;  // channels, groups, channels per group
   int tile_groups;    // groups per column tile
   float eps;
   int act;
-  float2* part;       // [chunks, 2, groups]: (mean, M2) of a long graph's piece: it began earlier / it begins here
-  float2* fin;        // [chunks, groups]: (mean, 1 / sqrt(var + eps)) of the long graph that begins in the chunk
-  int64_t chunks;
+  int window;         // rows per block (a multiple of kShort)
+  int64_t windows;
+  float2* part;       // [windows, 2, groups]: (mean, M2) of a split graph's piece: it began earlier / it begins here
+  float2* fin;        // [windows, groups]: (mean, 1 / sqrt(var + eps)) of the split graph that begins in the window
 };
 
-__device__ __forceinline__ float activate(float y, int act) {
+// erf by the rational approximation of Abramowitz and Stegun, Handbook of Mathematical
+// Functions, 7.1.26 (off by at most 1.5e-7), which needs one exponential.
+__device__ __forceinline__ float erf_as(float x) {
+  const float z = fabsf(x);
+  const float t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f));
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  return copysignf(fmaf(-p * t, __expf(-z * z), 1.0f), x);
+}
+
+template <int ACT>
+__device__ __forceinline__ float activate(float y) {
+  if constexpr (ACT == GNN_ACT_RELU) return y < 0.0f ? 0.0f : y;
+  if constexpr (ACT == GNN_ACT_SILU) return __fdividef(y, 1.0f + __expf(-y));
+  if constexpr (ACT == GNN_ACT_GELU) return 0.5f * y * (1.0f + erf_as(y * 0.70710678118654752f));
+  return y;
+}
+
+// Calls f with the activation as a compile-time constant.
+template <class F>
+__device__ __forceinline__ void with_activation(int act, F f) {
   switch (act) {
-    case GNN_ACT_RELU: return y < 0.0f ? 0.0f : y;
-    case GNN_ACT_SILU: return __fdividef(y, 1.0f + __expf(-y));
-    case GNN_ACT_GELU: return 0.5f * y * (1.0f + erff(y * 0.70710678118654752f));
-    default: return y;
+    case GNN_ACT_RELU: f(std::integral_constant<int, GNN_ACT_RELU>{}); break;
+    case GNN_ACT_SILU: f(std::integral_constant<int, GNN_ACT_SILU>{}); break;
+    case GNN_ACT_GELU: f(std::integral_constant<int, GNN_ACT_GELU>{}); break;
+    default: f(std::integral_constant<int, GNN_ACT_NONE>{}); break;
   }
 }
 
-template <class IdxT>
 __device__ __forceinline__ int64_t ptr_at(const NormArgs& a, int64_t g) {
-  const int64_t v = static_cast<int64_t>(__ldg(static_cast<const IdxT*>(a.ptr) + g));
+  const int64_t v = a.wide_ptr ? __ldg(static_cast<const int64_t*>(a.ptr) + g)
+                               : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(a.ptr) + g));
   return v < 0 ? 0 : (v > a.n ? a.n : v);
 }
 
-// The first graph whose end lies past `row` (graphs where there is none).
-template <class IdxT>
+// The first graph whose end lies past `row` (graphs where there is none): every lane
+// of the warp asks at another place, five bits a round.
 __device__ __forceinline__ int64_t graph_of(const NormArgs& a, int64_t row) {
-  int64_t lo = 0, hi = a.graphs;
+  const int lane = threadIdx.x & 31;
+  int64_t lo = 0, hi = a.graphs;  // the answer is in [lo, hi]
   while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (ptr_at<IdxT>(a, mid + 1) > row) {
-      hi = mid;
-    } else {
-      lo = mid + 1;
-    }
+    const int64_t step = (hi - lo + 31) / 32;
+    const int64_t at = min(lo + lane * step + step - 1, hi - 1);
+    const unsigned past = __ballot_sync(kFull, ptr_at(a, at + 1) > row);
+    if (past == 0) return hi;
+    const int first = __ffs(past) - 1;
+    hi = min(lo + first * step + step - 1, hi - 1);
+    lo = min(lo + first * step, hi);
+    if (step == 1) return hi;
   }
   return lo;
 }
 
 // A warp's view of one column tile: lane l holds the channels
-// c0 + CH * (l + 32 j) .. + CH, j < NV.
-template <int CH, int NV>
+// c0 + CH * (l + 32 j) .. + CH, j < NV. WHOLE: a chunk of CH channels lies in one
+// group. What belongs to a group is kept once a chunk (WHOLE) or once a channel.
+template <int CH, int NV, bool WHOLE>
 struct Tile {
+  static constexpr int E = WHOLE ? 1 : CH;
   int c0, cols;     // first channel, channels
   int g0, groups;   // first group, groups
   int cg;           // channels per group
-  int gsize;        // chunks of CH channels per group
   int lane;
-  bool pow2;        // a group is an aligned power of two of at most 32 lanes
-  int grp[NV];      // group (in the tile) of chunk lane + 32 j
-  float* sh;        // this warp's scratch: 32 NV partials and up to kTile totals
+  int gsize;        // WHOLE: chunks per group
+  bool pow2;        // WHOLE: a group is an aligned power of two of at most 32 lanes
+  int grp[NV];      // group (in the tile) of chunk lane + 32 j (of its first channel)
+  uint32_t delta[NV];  // !WHOLE: how many groups further channel e is, two bits each
+  float* sh;        // this warp's scratch: partials, totals
 
   __device__ __forceinline__ bool live(int j) const { return (lane + 32 * j) * CH < cols; }
   __device__ __forceinline__ int channel(int j) const { return c0 + CH * (lane + 32 * j); }
+  __device__ __forceinline__ int group(int j, int e) const {
+    return WHOLE ? grp[j] : grp[j] + static_cast<int>((delta[j] >> (2 * e)) & 3u);
+  }
+  // channel e of chunk j is the first of its group
+  __device__ __forceinline__ bool leads(int j, int e) const {
+    return WHOLE ? (lane + 32 * j) % gsize == 0 : CH * (lane + 32 * j) + e == group(j, e) * cg;
+  }
 
   __device__ __forceinline__ void init(const NormArgs& a, float* scratch) {
     lane = threadIdx.x & 31;
@@ -98,35 +141,53 @@ struct Tile {
     cg = a.cg;
     c0 = g0 * cg;
     cols = groups * cg;
-    gsize = cg / CH;
+    gsize = WHOLE ? cg / CH : 1;
     pow2 = gsize <= 32 && (gsize & (gsize - 1)) == 0;
     sh = scratch;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) grp[j] = (lane + 32 * j) / gsize;
+    for (int j = 0; j < NV; ++j) {
+      const int ch = CH * (lane + 32 * j);
+      grp[j] = ch / cg;
+      delta[j] = 0;
+      if constexpr (!WHOLE) {
+#pragma unroll
+        for (int e = 1; e < CH; ++e) delta[j] |= static_cast<uint32_t>((ch + e) / cg - grp[j]) << (2 * e);
+      }
+    }
   }
 
-  // p[j]: this lane's partial of chunk j -> the total of the chunk's group
-  __device__ __forceinline__ void group_sum(float (&p)[NV]) const {
-    if (pow2) {
+  // p[j][e]: this lane's partials -> the totals of their groups
+  __device__ __forceinline__ void group_sum(float (&p)[NV][E]) const {
+    if (WHOLE && pow2) {
       for (int o = 1; o < gsize; o <<= 1) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) p[j] += __shfl_xor_sync(kFull, p[j], o);
+        for (int j = 0; j < NV; ++j) p[j][0] += __shfl_xor_sync(kFull, p[j][0], o);
       }
       return;
     }
     if (groups == 1) {
       float s = 0.0f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) s += live(j) ? p[j] : 0.0f;
+      for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += live(j) ? p[j][e] : 0.0f;
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) p[j] = s;
+      for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) p[j][e] = s;
+      }
       return;
     }
-    float* tot = sh + 32 * NV;
+    const int each = WHOLE ? gsize : cg;  // partials per group
+    float* tot = sh + 32 * NV * E;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) sh[lane + 32 * j] = p[j];
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) sh[(lane + 32 * j) * E + e] = p[j][e];
+    }
     __syncwarp();
     int per = 1;  // lanes per group
     while (per * 2 * min(groups, 32) <= 32) per *= 2;
@@ -135,17 +196,26 @@ struct Tile {
       const int g = base + at;
       float s = 0.0f;
       if (g < groups) {
-        for (int i = t; i < gsize; i += per) s += sh[g * gsize + i];
+        for (int i = t; i < each; i += per) s += sh[g * each + i];
       }
       for (int o = 1; o < per; o <<= 1) s += __shfl_xor_sync(kFull, s, o);
       if (t == 0 && g < groups) tot[g] = s;
     }
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < NV; ++j) p[j] = live(j) ? tot[grp[j]] : 0.0f;
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) p[j][e] = live(j) ? tot[group(j, e)] : 0.0f;
+    }
     __syncwarp();
   }
 };
+
+// partials and totals of group_sum (at most a group per partial), per warp
+template <int CH, int NV, bool WHOLE>
+constexpr int scratch_floats() {
+  return 2 * 32 * NV * (WHOLE ? 1 : CH);
+}
 
 template <int CH>
 __device__ __forceinline__ void load_chunk(const float* p, float (&v)[CH]) {
@@ -169,8 +239,8 @@ __device__ __forceinline__ void store_chunk(float* p, const float (&v)[CH]) {
   }
 }
 
-template <int CH, int NV>
-__device__ __forceinline__ void load_affine(const NormArgs& a, const Tile<CH, NV>& t, float (&w)[NV][CH],
+template <int CH, int NV, bool WHOLE>
+__device__ __forceinline__ void load_affine(const NormArgs& a, const Tile<CH, NV, WHOLE>& t, float (&w)[NV][CH],
                                             float (&b)[NV][CH]) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -182,346 +252,566 @@ __device__ __forceinline__ void load_affine(const NormArgs& a, const Tile<CH, NV
   }
 }
 
-// 8 warps a block; 4 where their scratch would not fit the static 48 KB
-template <int NV>
-constexpr int block_warps() {
-  return NV >= 32 ? 4 : 8;
+// blocks per SM that the registers have to allow
+#ifndef NB
+#define NB 3
+#endif
+template <int CH, int NV>
+constexpr int min_blocks() {
+  return CH * NV <= 4 ? NB : (CH * NV <= 8 ? 2 : 1);
 }
 
-template <int CH, int NV>
-constexpr int scratch_floats() {
-  return 32 * NV + 32 * NV;  // partials, totals (at most one group per chunk)
-}
-
-// ---- each node on its own: one warp per row --------------------------------
-template <int CH, int NV>
-__global__ void __launch_bounds__(32 * block_warps<NV>()) norm_rows_kernel(NormArgs a) {
-  constexpr int kWarps = block_warps<NV>();
-  __shared__ float scratch[kWarps][scratch_floats<CH, NV>()];
-  Tile<CH, NV> t;
-  t.init(a, scratch[threadIdx.x >> 5]);
+// ---- each node on its own: one warp per row, R rows in flight ----------------
+template <int CH, int NV, bool WHOLE>
+__global__ void __launch_bounds__(kThreads, min_blocks<CH, NV>()) norm_rows_kernel(NormArgs a) {
+  constexpr int R = NV * CH <= 4 ? 4 : (NV * CH <= 8 ? 2 : 1);
+  constexpr int E = WHOLE ? 1 : CH;
+  extern __shared__ float scratch[];
+  Tile<CH, NV, WHOLE> t;
+  t.init(a, scratch + (threadIdx.x >> 5) * scratch_floats<CH, NV, WHOLE>());
   float w[NV][CH], b[NV][CH];
   load_affine(a, t, w, b);
   const float inv = 1.0f / static_cast<float>(a.cg);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); r < a.n; r += step) {
-    const float* src = a.x + r * a.c;
-    float v[NV][CH], p[NV];
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps * R;
+  for (int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * R; r0 < a.n; r0 += step) {
+    float v[R][NV][CH];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      p[j] = 0.0f;
-      if (t.live(j)) {
-        load_chunk<CH>(src + t.channel(j), v[j]);
+    for (int i = 0; i < R; ++i) {
 #pragma unroll
-        for (int e = 0; e < CH; ++e) p[j] += v[j][e];
+      for (int j = 0; j < NV; ++j) {
+        if (t.live(j) && r0 + i < a.n) load_chunk<CH>(a.x + (r0 + i) * a.c + t.channel(j), v[i][j]);
       }
     }
-    t.group_sum(p);
-    float q[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      q[j] = 0.0f;
-      if (t.live(j)) {
+    for (int i = 0; i < R; ++i) {
+      if (r0 + i >= a.n) break;
+      float p[NV][E];
 #pragma unroll
-        for (int e = 0; e < CH; ++e) {
-          v[j][e] -= p[j] * inv;
-          q[j] = fmaf(v[j][e], v[j][e], q[j]);
+      for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) p[j][e] = 0.0f;
+        if (t.live(j)) {
+#pragma unroll
+          for (int e = 0; e < CH; ++e) p[j][e % E] += v[i][j][e];
         }
       }
-    }
-    t.group_sum(q);
-    float* dst = a.out + r * a.c;
+      t.group_sum(p);
+      float q[NV][E];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (t.live(j)) {
-        const float rstd = __frcp_rn(__fsqrt_rn(fmaf(q[j], inv, a.eps)));
+      for (int j = 0; j < NV; ++j) {
 #pragma unroll
-        for (int e = 0; e < CH; ++e) v[j][e] = activate(fmaf(v[j][e] * rstd, w[j][e], b[j][e]), a.act);
-        store_chunk<CH>(dst + t.channel(j), v[j]);
+        for (int e = 0; e < E; ++e) q[j][e] = 0.0f;
+        if (t.live(j)) {
+#pragma unroll
+          for (int e = 0; e < CH; ++e) {
+            v[i][j][e] -= p[j][e % E] * inv;
+            q[j][e % E] = fmaf(v[i][j][e], v[i][j][e], q[j][e % E]);
+          }
+        }
       }
+      t.group_sum(q);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (t.live(j)) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) q[j][e] = __frcp_rn(__fsqrt_rn(fmaf(q[j][e], inv, a.eps)));
+#pragma unroll
+          for (int e = 0; e < CH; ++e) v[i][j][e] = fmaf(v[i][j][e] * q[j][e % E], w[j][e], b[j][e]);
+        }
+      }
+      with_activation(a.act, [&](auto act) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          if (t.live(j)) {
+#pragma unroll
+            for (int e = 0; e < CH; ++e) v[i][j][e] = activate<decltype(act)::value>(v[i][j][e]);
+            store_chunk<CH>(a.out + (r0 + i) * a.c + t.channel(j), v[i][j]);
+          }
+        }
+      });
     }
   }
 }
 
 // ---- graphs of a batch ------------------------------------------------------
 
-template <int NV>
+// rows of a warp in flight
+template <int CH, int NV>
 constexpr int batch_rows() {
-  return NV == 1 ? 8 : (NV == 2 ? 4 : (NV <= 8 ? 2 : 1));
+  return NV * CH <= 4 ? 8 : (NV * CH <= 8 ? 4 : (NV * CH <= 16 ? 2 : 1));
 }
 
-// (mean, M2) per group of rows [beg, end), in the lanes of the group's chunks.
-template <int CH, int NV>
-__device__ __forceinline__ void piece_stats(const NormArgs& a, const Tile<CH, NV>& t, int64_t beg, int64_t end,
-                                            float (&mean)[NV], float (&m2)[NV]) {
-  constexpr int U = batch_rows<NV>();
-  float m[NV][CH], s[NV][CH];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-#pragma unroll
-    for (int e = 0; e < CH; ++e) m[j][e] = s[j][e] = 0.0f;
-  }
-  float n = 0.0f;
-  for (int64_t r = beg; r < end; r += U) {
-    float v[U][NV][CH];
-    const int cnt = static_cast<int>(min(static_cast<int64_t>(U), end - r));
+// The rows of a span, shared by a team: warp i of `size` takes rows i, i + size, ...
+// The team is the block, or a warp by itself.
+template <int CH, int NV, bool WHOLE>
+struct Team {
+  static constexpr int E = WHOLE ? 1 : CH;
+  static constexpr int U = batch_rows<CH, NV>();
+  Tile<CH, NV, WHOLE> t;
+  float2* joint;  // [2][kWarps][groups in the tile]: (mean, M2) of the warps' rows
+  int flip;       // which half of `joint` is next
+  int size;       // kWarps or 1
+  int warp;       // this warp's place in the team
+  float v[U][NV][CH];
+
+  __device__ __forceinline__ int keep() const { return size * U; }  // rows that stay in registers
+
+  // every size-th of `rows` rows
+  __device__ __forceinline__ int count(int rows) const { return size == 1 ? rows : (rows + kWarps - 1) / kWarps; }
+
+  // rows first + size u of [first, end), as many as there are
+  __device__ __forceinline__ int load(const NormArgs& a, int64_t first, int64_t end) {
+    const int cnt = first < end ? min(U, count(static_cast<int>(end - first))) : 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (u < cnt && t.live(j)) {
-          load_chunk<CH>(a.x + (r + u) * a.c + t.channel(j), v[u][j]);
+          load_chunk<CH>(a.x + (first + u * size) * a.c + t.channel(j), v[u][j]);
         } else {
 #pragma unroll
           for (int e = 0; e < CH; ++e) v[u][j][e] = 0.0f;
         }
       }
     }
-    const float cf = static_cast<float>(cnt);
-    const float icf = __frcp_rn(cf);
-    const float nn = n + cf;
-    const float share = __fdividef(cf, nn);
-    const float both = n * share;
+    return cnt;
+  }
+
+  // (mean, M2) of the groups over rows [beg, end), the same in every warp; one batch of
+  // rows is left in v
+  __device__ __forceinline__ void stats(const NormArgs& a, int64_t beg, int64_t end, float (&mean)[NV][E],
+                                        float (&m2)[NV][E]) {
+    float m[NV][CH], s[NV][CH];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
 #pragma unroll
-      for (int e = 0; e < CH; ++e) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int u = 0; u < U; ++u) sum += v[u][j][e];
-        const float mb = sum * icf;
-        float dev = 0.0f;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float d = v[u][j][e] - mb;
-          if (u < cnt) dev = fmaf(d, d, dev);
-        }
-        const float delta = mb - m[j][e];
-        m[j][e] = fmaf(delta, share, m[j][e]);
-        s[j][e] += fmaf(delta * delta, both, dev);
-      }
+      for (int e = 0; e < CH; ++e) m[j][e] = s[j][e] = 0.0f;
     }
-    n = nn;
-  }
-  // channels of a group: n values each
-  const float icg = 1.0f / static_cast<float>(a.cg);
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    mean[j] = 0.0f;
-    if (t.live(j)) {
-#pragma unroll
-      for (int e = 0; e < CH; ++e) mean[j] += m[j][e];
-    }
-  }
-  t.group_sum(mean);
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    mean[j] *= icg;
-    m2[j] = 0.0f;
-    if (t.live(j)) {
-#pragma unroll
-      for (int e = 0; e < CH; ++e) {
-        const float d = m[j][e] - mean[j];
-        m2[j] += fmaf(d * d, n, s[j][e]);
-      }
-    }
-  }
-  t.group_sum(m2);
-}
-
-// Rows [beg, end) with the statistics of their groups.
-template <int CH, int NV>
-__device__ __forceinline__ void apply_rows(const NormArgs& a, const Tile<CH, NV>& t, int64_t beg, int64_t end,
-                                           const float (&mean)[NV], const float (&rstd)[NV]) {
-  constexpr int U = batch_rows<NV>() >= 4 ? 4 : batch_rows<NV>();
-  float w[NV][CH], b[NV][CH];
-  load_affine(a, t, w, b);
-  for (int64_t r = beg; r < end; r += U) {
-    float v[U][NV][CH];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
+    float n = 0.0f;
+    for (int64_t r = beg; r < end; r += keep()) {
+      const int cnt = load(a, r + warp, end);
+      if (cnt == 0) break;
+      const float cf = static_cast<float>(cnt);
+      const float icf = __frcp_rn(cf);
+      const float nn = n + cf;
+      const float share = __fdividef(cf, nn);
+      const float both = n * share;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (r + u < end && t.live(j)) load_chunk<CH>(a.x + (r + u) * a.c + t.channel(j), v[u][j]);
-      }
-    }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+        for (int e = 0; e < CH; ++e) {
+          float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (r + u < end && t.live(j)) {
+          for (int u = 0; u < U; ++u) sum += v[u][j][e];
+          const float mb = sum * icf;
+          float dev = 0.0f;
 #pragma unroll
-          for (int e = 0; e < CH; ++e) {
-            v[u][j][e] = activate(fmaf((v[u][j][e] - mean[j]) * rstd[j], w[j][e], b[j][e]), a.act);
+          for (int u = 0; u < U; ++u) {
+            if (u < cnt) {
+              const float d = v[u][j][e] - mb;
+              dev = fmaf(d, d, dev);
+            }
           }
-          store_chunk<CH>(a.out + (r + u) * a.c + t.channel(j), v[u][j]);
+          const float d = mb - m[j][e];
+          m[j][e] = fmaf(d, share, m[j][e]);
+          s[j][e] += fmaf(d * d, both, dev);
+        }
+      }
+      n = nn;
+    }
+    // the channels of a group: n values each
+    const float icg = 1.0f / static_cast<float>(a.cg);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) mean[j][e] = 0.0f;
+      if (t.live(j)) {
+#pragma unroll
+        for (int e = 0; e < CH; ++e) mean[j][e % E] += m[j][e];
+      }
+    }
+    t.group_sum(mean);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        mean[j][e] *= icg;
+        m2[j][e] = 0.0f;
+      }
+      if (t.live(j)) {
+#pragma unroll
+        for (int e = 0; e < CH; ++e) {
+          const float d = m[j][e] - mean[j][e % E];
+          m2[j][e % E] += fmaf(d * d, n, s[j][e]);
+        }
+      }
+    }
+    t.group_sum(m2);
+    if (size == 1) return;
+    // the warps: warp i has the rows beg + i, beg + i + 8, ...
+    const int stride = a.tile_groups;
+    float2* half = joint + flip * kWarps * stride;
+    flip ^= 1;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (t.live(j) && t.leads(j, e)) half[warp * stride + t.group(j, e)] = make_float2(mean[j][e], m2[j][e]);
+      }
+    }
+    __syncthreads();
+    const int64_t rows = end - beg;
+    const float inv = 1.0f / static_cast<float>(rows);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (!t.live(j)) continue;
+        const float2* p = half + t.group(j, e);
+        float sum = 0.0f, dev = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+          const float ni = static_cast<float>((rows - i + kWarps - 1) / kWarps);
+          if (i < rows) sum = fmaf(ni, p[i * stride].x, sum);
+        }
+        const float mu = sum * inv;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+          const float ni = static_cast<float>((rows - i + kWarps - 1) / kWarps) * static_cast<float>(a.cg);
+          const float d = p[i * stride].x - mu;
+          if (i < rows) dev += fmaf(d * d, ni, p[i * stride].y);
+        }
+        mean[j][e] = mu;
+        m2[j][e] = dev;
+      }
+    }
+  }
+
+  // normalises and stores the batch in v: rows first + 8 u
+  __device__ __forceinline__ void put(const NormArgs& a, int64_t first, int cnt, const float (&mean)[NV][E],
+                                      const float (&rstd)[NV][E], const float (&w)[NV][CH],
+                                      const float (&b)[NV][CH]) {
+with_activation(a.act, [&](auto act) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (u >= cnt) break;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          if (t.live(j)) {
+#pragma unroll
+            for (int e = 0; e < CH; ++e) {
+              v[u][j][e] = activate<decltype(act)::value>(
+                  fmaf((v[u][j][e] - mean[j][e % E]) * rstd[j][e % E], w[j][e], b[j][e]));
+            }
+            store_chunk<CH>(a.out + (first + u * size) * a.c + t.channel(j), v[u][j]);
+          }
+        }
+      }
+    });
+  }
+
+  __device__ __forceinline__ void init(const NormArgs& a, float* shared) {
+    warp = threadIdx.x >> 5;
+    size = kWarps;
+    flip = 0;
+    joint = reinterpret_cast<float2*>(shared);
+    t.init(a, shared + 4 * kWarps * a.tile_groups + warp * scratch_floats<CH, NV, WHOLE>());
+  }
+};
+
+// The graphs of a window. Short: at most kShort rows, starts here (and may run on into
+// the next window). Long: more rows; whole ones lie inside the window, split ones
+// (at most two of them) do not.
+struct Window {
+  int shorts, longs, next;
+  int item[kMaxWindow];  // short: first row from r0 << 8 | rows
+  int64_t begin[kMaxLongs], end[kMaxLongs];
+};
+
+__device__ __forceinline__ bool is_split(const NormArgs& a, int64_t s, int64_t e) {
+  return e - s > kShort && s / a.window != (e - 1) / a.window;
+}
+
+// Lists the graphs of rows [r0, r1) (in any order: no result depends on it); of the
+// long ones only the split ones where `split_only`.
+__device__ __forceinline__ void list_graphs(const NormArgs& a, int64_t r0, int64_t r1, bool split_only, Window& w) {
+  if (threadIdx.x == 0) w.shorts = w.longs = w.next = 0;
+  __syncthreads();
+  const int64_t last = graph_of(a, r1 - 1);
+  for (int64_t g = graph_of(a, r0) + threadIdx.x; g <= last && g < a.graphs; g += kThreads) {
+    const int64_t s = ptr_at(a, g), e = ptr_at(a, g + 1);
+    if (e - s > kShort && s < r1 && e > r0) {
+      if (split_only && !is_split(a, s, e)) continue;
+      const int i = atomicAdd(&w.longs, 1);
+      if (i < kMaxLongs) {
+        w.begin[i] = s;
+        w.end[i] = e;
+      }
+    } else if (!split_only && e > s && e - s <= kShort && s >= r0 && s < r1) {
+      const int i = atomicAdd(&w.shorts, 1);
+      if (i < kMaxWindow) w.item[i] = static_cast<int>(s - r0) << 8 | static_cast<int>(e - s);
+    }
+  }
+  __syncthreads();
+}
+
+template <int CH, int NV, bool WHOLE>
+__global__ void __launch_bounds__(kThreads, min_blocks<CH, NV>()) norm_windows_kernel(NormArgs a) {
+  constexpr int E = WHOLE ? 1 : CH;
+  extern __shared__ float shared[];
+  __shared__ Window list;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.window, r1 = min(r0 + a.window, a.n);
+  list_graphs(a, r0, r1, false, list);
+  Team<CH, NV, WHOLE> team;
+  team.init(a, shared);
+  const int me = team.warp;
+  float w[NV][CH], b[NV][CH];
+  load_affine(a, team.t, w, b);
+  float mean[NV][E], m2[NV][E];
+  // normalises rows [s, e), whose statistics are (mean, m2)
+  auto finish = [&](int64_t s, int64_t e) {
+    const int rows = static_cast<int>(e - s);
+    const float inv = 1.0f / (static_cast<float>(rows) * static_cast<float>(a.cg));
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int k = 0; k < E; ++k) m2[j][k] = __frcp_rn(__fsqrt_rn(fmaf(m2[j][k], inv, a.eps)));
+    }
+    const bool kept = rows <= team.keep();  // they are still in registers
+    for (int64_t r = s + team.warp; r < e; r += team.keep()) {
+      const int cnt = kept ? team.count(static_cast<int>(e - r)) : team.load(a, r, e);
+      team.put(a, r, cnt, mean, m2, w, b);
+    }
+  };
+  // Several short graphs: each warp takes one after the other by itself. Few: all
+  // warps work on each.
+  const int shorts = min(list.shorts, kMaxWindow);
+  const bool solo = shorts >= kWarps / 2;
+  if (solo) {
+    team.size = 1;
+    team.warp = 0;
+  }
+  for (int i = 0;; ++i) {
+    if (solo) {
+      if (team.t.lane == 0) i = atomicAdd(&list.next, 1);
+      i = __shfl_sync(kFull, i, 0);
+    }
+    if (i >= shorts) break;
+    const int item = list.item[i];
+    const int64_t s = r0 + (item >> 8), e = s + (item & 0xff);
+    team.stats(a, s, e, mean, m2);
+    finish(s, e);
+  }
+  team.size = kWarps;
+  team.warp = me;
+  const int longs = min(list.longs, kMaxLongs);
+  for (int i = 0; i < longs; ++i) {
+    const int64_t s = list.begin[i], e = list.end[i];
+    team.stats(a, max(s, r0), min(e, r1), mean, m2);
+    if (!is_split(a, s, e)) {
+      finish(s, e);
+    } else if (me == 0) {
+      float2* slot = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (s >= r0 ? 1 : 0)) * a.groups + team.t.g0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+          if (team.t.live(j) && team.t.leads(j, k)) slot[team.t.group(j, k)] = make_float2(mean[j][k], m2[j][k]);
         }
       }
     }
   }
 }
 
-template <int CH, int NV, class IdxT>
-__global__ void __launch_bounds__(32 * block_warps<NV>()) norm_pieces_kernel(NormArgs a) {
-  constexpr int kWarps = block_warps<NV>();
-  __shared__ float scratch[kWarps][scratch_floats<CH, NV>()];
-  Tile<CH, NV> t;
-  t.init(a, scratch[threadIdx.x >> 5]);
-  const int64_t chunk = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (chunk >= a.chunks) return;
-  const int64_t r0 = chunk * kChunk, r1 = min(r0 + kChunk, a.n);
-  for (int64_t g = graph_of<IdxT>(a, r0); g < a.graphs;) {
-    const int64_t s = ptr_at<IdxT>(a, g), e = ptr_at<IdxT>(a, g + 1);
-    if (s >= r1) break;
-    float mean[NV], m2[NV];
-    if (e - s <= kChunk) {
-      if (s >= r0 && e > s) {
-        piece_stats<CH, NV>(a, t, s, e, mean, m2);
-        const float inv = 1.0f / (static_cast<float>(e - s) * static_cast<float>(a.cg));
-#pragma unroll
-        for (int j = 0; j < NV; ++j) m2[j] = __frcp_rn(__fsqrt_rn(fmaf(m2[j], inv, a.eps)));
-        apply_rows<CH, NV>(a, t, s, e, mean, m2);
-      }
-    } else {
-      piece_stats<CH, NV>(a, t, max(s, r0), min(e, r1), mean, m2);
-      float2* slot = a.part + (chunk * 2 + (s >= r0 ? 1 : 0)) * a.groups + t.g0;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        // the first chunk of a group writes for all of it
-        if (t.live(j) && (t.lane + 32 * j) % t.gsize == 0) slot[t.grp[j]] = make_float2(mean[j], m2[j]);
-      }
-    }
-    ++g;
-    // a run of empty graphs is passed in one search
-    if (g < a.graphs && ptr_at<IdxT>(a, g + 1) <= e) g = max(g, graph_of<IdxT>(a, max(e, r0)));
+// The pieces of a split graph, one per window.
+struct Pieces {
+  int64_t s, e, first, last;  // rows [s, e), windows first .. last
+  double total;               // values per group
+  __device__ __forceinline__ Pieces(const NormArgs& a, int64_t g)
+      : s(ptr_at(a, g)), e(ptr_at(a, g + 1)), first(s / a.window), last((e - 1) / a.window),
+        total(static_cast<double>(e - s) * a.cg) {}
+  // values per group of piece k
+  __device__ __forceinline__ double size(const NormArgs& a, int64_t k) const {
+    return static_cast<double>(min(e, (k + 1) * a.window) - max(s, k * a.window)) * a.cg;
   }
-}
+  __device__ __forceinline__ float2 at(const NormArgs& a, int64_t k, int grp) const {
+    return a.part[(k * 2 + (k == first ? 1 : 0)) * a.groups + grp];
+  }
+  __device__ __forceinline__ void put(const NormArgs& a, int grp, double mean, double m2) const {
+    a.fin[first * a.groups + grp] =
+        make_float2(static_cast<float>(mean), static_cast<float>(1.0 / sqrt(m2 / total + a.eps)));
+  }
+};
 
-__device__ __forceinline__ double block_sum(double v, double* sh) {
+__device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  double s = 0.0;
-#pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; ++i) s += sh[i];
-  __syncthreads();
-  return s;
+  return v;
 }
 
-// Joins the pieces of long graphs, in 64 bits and in piece order per thread:
-// blocks take graphs in batches of kJoinThreads, group by group (blockIdx.y, striding).
-template <class IdxT>
-__global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(NormArgs a) {
-  __shared__ double sh[kJoinThreads / 32];
-  __shared__ int todo[kJoinThreads];
-  __shared__ int count;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kJoinThreads; base < a.graphs;
-       base += static_cast<int64_t>(gridDim.x) * kJoinThreads) {
-    if (threadIdx.x == 0) count = 0;
-    __syncthreads();
-    const int64_t mine = base + threadIdx.x;
-    if (mine < a.graphs && ptr_at<IdxT>(a, mine + 1) - ptr_at<IdxT>(a, mine) > kChunk) {
-      todo[atomicAdd(&count, 1)] = threadIdx.x;  // the order of graphs does not touch their results
+// Joins the pieces of split graphs in 64 bits, always in the same order. Blocks with
+// blockIdx.y == 0 look through the graphs, 32 a warp at a time, and join those of few
+// pieces, a warp each; the others take the graphs of many pieces, a block per group.
+__global__ void __launch_bounds__(kThreads) norm_join_kernel(NormArgs a) {
+  __shared__ double sh[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool few = blockIdx.y == 0;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * (few ? kThreads : 32);
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * (few ? kThreads : 32) + (few ? warp * 32 : 0);
+       base < a.graphs; base += stride) {
+    bool mine = false;
+    if (base + lane < a.graphs) {
+      const int64_t s = ptr_at(a, base + lane), e = ptr_at(a, base + lane + 1);
+      const bool many = e - s > static_cast<int64_t>(kFewPieces - 2) * a.window;
+      mine = is_split(a, s, e) && many != few;
     }
-    __syncthreads();
-    for (int i = 0; i < count; ++i) {
-      const int64_t g = base + todo[i];
-      const int64_t s = ptr_at<IdxT>(a, g), e = ptr_at<IdxT>(a, g + 1);
-      const int64_t first = s / kChunk, last = (e - 1) / kChunk;
-      const double total = static_cast<double>(e - s) * a.cg;
-      for (int grp = blockIdx.y; grp < a.groups; grp += gridDim.y) {
-        double sum = 0.0;
-        for (int64_t k = first + threadIdx.x; k <= last; k += kJoinThreads) {
-          const int64_t rows = min(e, (k + 1) * kChunk) - max(s, k * kChunk);
-          const float2 p = a.part[(k * 2 + (k == first ? 1 : 0)) * a.groups + grp];
-          sum += static_cast<double>(rows) * a.cg * p.x;
+    for (unsigned todo = __ballot_sync(kFull, mine); todo != 0; todo &= todo - 1) {
+      const Pieces p(a, base + __ffs(todo) - 1);
+      if (few) {  // at most kFewPieces pieces
+        for (int grp = 0; grp < a.groups; ++grp) {
+          float2 v[2];
+          double size[2], sum = 0.0, m2 = 0.0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int64_t k = p.first + lane + 32 * i;
+            v[i] = k <= p.last ? p.at(a, k, grp) : make_float2(0.0f, 0.0f);
+            size[i] = k <= p.last ? p.size(a, k) : 0.0;
+            sum += size[i] * v[i].x;
+          }
+          const double mean = warp_sum(sum) / p.total;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) m2 += v[i].y + size[i] * (v[i].x - mean) * (v[i].x - mean);
+          m2 = warp_sum(m2);
+          if (lane == 0) p.put(a, grp, mean, m2);
         }
-        const double mean = block_sum(sum, sh) / total;
-        double m2 = 0.0;
-        for (int64_t k = first + threadIdx.x; k <= last; k += kJoinThreads) {
-          const int64_t rows = min(e, (k + 1) * kChunk) - max(s, k * kChunk);
-          const float2 p = a.part[(k * 2 + (k == first ? 1 : 0)) * a.groups + grp];
-          const double d = p.x - mean;
-          m2 += p.y + static_cast<double>(rows) * a.cg * d * d;
-        }
-        m2 = block_sum(m2, sh);
-        if (threadIdx.x == 0) {
-          a.fin[first * a.groups + grp] =
-              make_float2(static_cast<float>(mean), static_cast<float>(1.0 / sqrt(m2 / total + a.eps)));
+      } else {
+        for (int grp = blockIdx.y - 1; grp < a.groups; grp += gridDim.y - 1) {
+          auto block_sum = [&](double v) {
+            v = warp_sum(v);
+            if (lane == 0) sh[warp] = v;
+            __syncthreads();
+            double t = 0.0;
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) t += sh[i];
+            __syncthreads();
+            return t;
+          };
+          double sum = 0.0, m2 = 0.0;
+#pragma unroll 4
+          for (int64_t k = p.first + threadIdx.x; k <= p.last; k += kThreads) sum += p.size(a, k) * p.at(a, k, grp).x;
+          const double mean = block_sum(sum) / p.total;
+#pragma unroll 4
+          for (int64_t k = p.first + threadIdx.x; k <= p.last; k += kThreads) {
+            const float2 v = p.at(a, k, grp);
+            m2 += v.y + p.size(a, k) * (v.x - mean) * (v.x - mean);
+          }
+          m2 = block_sum(m2);
+          if (threadIdx.x == 0) p.put(a, grp, mean, m2);
         }
       }
     }
-    __syncthreads();
   }
 }
 
-// The rows of long graphs. A chunk holds at most two of them: the graph of its first
-// row and that of its last.
-template <int CH, int NV, class IdxT>
-__global__ void __launch_bounds__(32 * block_warps<NV>()) norm_apply_kernel(NormArgs a) {
-  constexpr int kWarps = block_warps<NV>();
-  __shared__ float scratch[kWarps][scratch_floats<CH, NV>()];
-  Tile<CH, NV> t;
-  t.init(a, scratch[threadIdx.x >> 5]);
-  const int64_t chunk = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (chunk >= a.chunks) return;
-  const int64_t r0 = chunk * kChunk, r1 = min(r0 + kChunk, a.n);
-  int64_t before = -1;
-  for (int i = 0; i < 2; ++i) {
-    const int64_t g = graph_of<IdxT>(a, i == 0 ? r0 : r1 - 1);
-    if (g >= a.graphs || g == before) continue;
-    before = g;
-    const int64_t s = ptr_at<IdxT>(a, g), e = ptr_at<IdxT>(a, g + 1);
-    if (e - s <= kChunk || s >= r1 || e <= r0) continue;
-    const float2* fin = a.fin + (s / kChunk) * a.groups + t.g0;
-    float mean[NV], rstd[NV];
+// The rows of split graphs; the last windows first, whose rows the L2 may still hold.
+template <int CH, int NV, bool WHOLE>
+__global__ void __launch_bounds__(kThreads, min_blocks<CH, NV>()) norm_apply_kernel(NormArgs a) {
+  constexpr int E = WHOLE ? 1 : CH;
+  extern __shared__ float shared[];
+  __shared__ Window list;
+  const int64_t r0 = (a.windows - 1 - blockIdx.x) * a.window, r1 = min(r0 + a.window, a.n);
+  list_graphs(a, r0, r1, true, list);
+  if (list.longs == 0) return;
+  Team<CH, NV, WHOLE> team;
+  team.init(a, shared);
+  float w[NV][CH], b[NV][CH];
+  load_affine(a, team.t, w, b);
+  for (int i = 0; i < min(list.longs, kMaxLongs); ++i) {
+    const int64_t s = list.begin[i];
+    const float2* fin = a.fin + (s / a.window) * a.groups + team.t.g0;
+    float mean[NV][E], rstd[NV][E];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const float2 f = t.live(j) ? fin[t.grp[j]] : make_float2(0.0f, 0.0f);
-      mean[j] = f.x;
-      rstd[j] = f.y;
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        const float2 f = team.t.live(j) ? fin[team.t.group(j, k)] : make_float2(0.0f, 0.0f);
+        mean[j][k] = f.x;
+        rstd[j][k] = f.y;
+      }
     }
-    apply_rows<CH, NV>(a, t, max(s, r0), min(e, r1), mean, rstd);
+    const int64_t beg = max(s, r0), end = min(list.end[i], r1);
+    for (int64_t r = beg + team.warp; r < end; r += team.keep()) {
+      team.put(a, r, team.load(a, r, end), mean, rstd, w, b);
+    }
   }
+}
+
+// Opts a kernel in to more than 48 KB of dynamic shared memory where it needs it.
+template <class Kernel>
+int allow_shared(Kernel kernel, size_t bytes) {
+  if (bytes <= 48 * 1024) return GNN_OK;
+  GNN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)),
+               "group norm: shared memory opt-in");
+  return GNN_OK;
 }
 
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
-int64_t chunks_for(int64_t n) { return (n + kChunk - 1) / kChunk; }
 
-size_t workspace_for(int64_t n, int64_t groups) {
-  if (n <= kChunk) return 0;  // every graph is finished by one warp
-  return static_cast<size_t>(round_up(chunks_for(n) * 3 * groups * 8, 256));
+// Rows per block: about eight graphs of average length, so that each warp has one to
+// itself (or, of long graphs, few pieces to join), as long as the SMs get a few blocks each.
+int window_for(int64_t n, int64_t graphs) {
+  int window = kShort;
+  while (window < kMaxWindow && window < 8 * (n / graphs) && n / (2 * window) >= 4 * sm_count()) window *= 2;
+  return window;
 }
 
-template <int CH, int NV, class IdxT>
-int run_batch(const NormArgs& a, unsigned tiles, cudaStream_t s) {
-  constexpr int kWarps = block_warps<NV>();
-  const dim3 grid(static_cast<unsigned>((a.chunks + kWarps - 1) / kWarps), tiles);
-  norm_pieces_kernel<CH, NV, IdxT><<<grid, 32 * kWarps, 0, s>>>(a);
-  GNN_LAUNCH_CHECK("norm_pieces_kernel launch");
-  if (a.n <= kChunk) return GNN_OK;
-  const int64_t batches = (a.graphs + kJoinThreads - 1) / kJoinThreads;
+size_t workspace_for(int64_t n, int64_t graphs, int64_t groups) {
+  if (n <= kShort) return 0;  // every graph is finished by one block
+  const int64_t window = window_for(n, graphs);
+  return static_cast<size_t>(round_up((n + window - 1) / window * 3 * groups * 8, 256));
+}
+
+template <int CH, int NV, bool WHOLE>
+int run(const NormArgs& a, bool rows, unsigned tiles, cudaStream_t s) {
+  const size_t warps = sizeof(float) * kWarps * scratch_floats<CH, NV, WHOLE>();
+  if (rows) {
+    constexpr int R = NV * CH <= 4 ? 4 : (NV * CH <= 8 ? 2 : 1);
+    const int64_t want = (a.n + kWarps * R - 1) / (kWarps * R);
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(want, 16LL * sm_count())), tiles);
+    if (int rc = allow_shared(norm_rows_kernel<CH, NV, WHOLE>, warps)) return rc;
+    norm_rows_kernel<CH, NV, WHOLE><<<grid, kThreads, warps, s>>>(a);
+    GNN_LAUNCH_CHECK("norm_rows_kernel launch");
+    return GNN_OK;
+  }
+  const size_t smem = warps + sizeof(float2) * 2 * kWarps * a.tile_groups;
+  const dim3 grid(static_cast<unsigned>(a.windows), tiles);
+  if (int rc = allow_shared(norm_windows_kernel<CH, NV, WHOLE>, smem)) return rc;
+  norm_windows_kernel<CH, NV, WHOLE><<<grid, kThreads, smem, s>>>(a);
+  GNN_LAUNCH_CHECK("norm_windows_kernel launch");
+  if (a.n <= kShort) return GNN_OK;
+  const int64_t batches = (a.graphs + kThreads - 1) / kThreads;
+  const bool many = a.n > static_cast<int64_t>(kFewPieces - 2) * a.window;  // some graph may have many pieces
   const dim3 jgrid(static_cast<unsigned>(std::min<int64_t>(batches, 4LL * sm_count())),
-                   static_cast<unsigned>(std::min(a.groups, 32)));
-  norm_join_kernel<IdxT><<<jgrid, kJoinThreads, 0, s>>>(a);
+                   many ? 1u + static_cast<unsigned>(std::min(a.groups, 64)) : 1u);
+  norm_join_kernel<<<jgrid, kThreads, 0, s>>>(a);
   GNN_LAUNCH_CHECK("norm_join_kernel launch");
-  norm_apply_kernel<CH, NV, IdxT><<<grid, 32 * kWarps, 0, s>>>(a);
+  if (int rc = allow_shared(norm_apply_kernel<CH, NV, WHOLE>, smem)) return rc;
+  norm_apply_kernel<CH, NV, WHOLE><<<grid, kThreads, smem, s>>>(a);
   GNN_LAUNCH_CHECK("norm_apply_kernel launch");
   return GNN_OK;
 }
 
-template <int CH, int NV>
-int run(const NormArgs& a, bool rows, bool wide_index, unsigned tiles, cudaStream_t s) {
-  if (rows) {
-    constexpr int kWarps = block_warps<NV>();
-    const int64_t want = (a.n + kWarps - 1) / kWarps;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(want, 16LL * sm_count())), tiles);
-    norm_rows_kernel<CH, NV><<<grid, 32 * kWarps, 0, s>>>(a);
-    GNN_LAUNCH_CHECK("norm_rows_kernel launch");
-    return GNN_OK;
+template <int CH, bool WHOLE>
+int run_width(const NormArgs& a, bool rows, int64_t cols, unsigned tiles, cudaStream_t s) {
+  if (cols <= 32 * CH) return run<CH, 1, WHOLE>(a, rows, tiles, s);
+  if (cols <= 64 * CH) return run<CH, 2, WHOLE>(a, rows, tiles, s);
+  if (cols <= 128 * CH) return run<CH, 4, WHOLE>(a, rows, tiles, s);
+  if (cols <= 256 * CH) return run<CH, 8, WHOLE>(a, rows, tiles, s);
+  if constexpr (CH == 1) {
+    if (cols <= 512) return run<CH, 16, WHOLE>(a, rows, tiles, s);
+    return run<CH, 32, WHOLE>(a, rows, tiles, s);
   }
-  return wide_index ? run_batch<CH, NV, int64_t>(a, tiles, s) : run_batch<CH, NV, int32_t>(a, tiles, s);
+  return fail(GNN_ERR_UNSUPPORTED, "group norm: column tile too wide");
 }
 
 }  // namespace
@@ -531,7 +821,7 @@ using namespace gnnb200;
 
 extern "C" size_t gnn_group_norm_workspace_bytes(int64_t num_nodes, int64_t num_graphs, int64_t groups) {
   if (num_nodes <= 0 || num_graphs <= 0 || groups <= 0) return 0;
-  return workspace_for(num_nodes, groups);
+  return workspace_for(num_nodes, num_graphs, groups);
 }
 
 extern "C" int gnn_group_norm_forward(const float* x, const void* graph_ptr, int graph_ptr_type, int64_t num_graphs,
@@ -558,7 +848,7 @@ extern "C" int gnn_group_norm_forward(const float* x, const void* graph_ptr, int
   GNN_REQUIRE(channels <= 0x7fffffffLL && tiles <= 65535, GNN_ERR_UNSUPPORTED, "too many channels");
   GNN_REQUIRE(num_nodes <= (int64_t(1) << 36), GNN_ERR_UNSUPPORTED, "too many nodes");
   GNN_REQUIRE(x != nullptr && out != nullptr, GNN_ERR_NULL_POINTER, "x and out must not be NULL");
-  const size_t need = graph_ptr != nullptr ? workspace_for(num_nodes, groups) : 0;
+  const size_t need = graph_ptr != nullptr ? workspace_for(num_nodes, num_graphs, groups) : 0;
   GNN_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), GNN_ERR_WORKSPACE,
               "workspace missing or too small (gnn_group_norm_workspace_bytes)");
   GNN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, GNN_ERR_WORKSPACE,
@@ -577,34 +867,27 @@ extern "C" int gnn_group_norm_forward(const float* x, const void* graph_ptr, int
   a.tile_groups = static_cast<int>(tile_groups);
   a.eps = eps;
   a.act = activation;
-  a.chunks = chunks_for(num_nodes);
-  a.part = static_cast<float2*>(workspace);
-  a.fin = a.part + a.chunks * 2 * groups;
-  const bool vec = cg % 4 == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  const int64_t cols = tile_groups * cg;
+  a.wide_ptr = graph_ptr_type == GNN_INDEX_INT64 ? 1 : 0;
   const bool rows = graph_ptr == nullptr;
-  const bool wide = graph_ptr_type == GNN_INDEX_INT64;
+  if (!rows) {
+    a.window = window_for(num_nodes, num_graphs);
+    a.windows = (num_nodes + a.window - 1) / a.window;
+    a.part = static_cast<float2*>(workspace);
+    a.fin = a.part + a.windows * 2 * groups;
+  }
+  // 16-byte pieces of rows: in several column tiles only where each starts on one
+  const bool vec = channels % 4 == 0 && (tiles == 1 || cg % 4 == 0) &&
+                   ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  const int64_t cols = tile_groups * cg;
   const unsigned ty = static_cast<unsigned>(tiles);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int rc;
-  if (vec) {
-    if (cols <= 128) {
-      rc = run<4, 1>(a, rows, wide, ty, s);
-    } else if (cols <= 256) {
-      rc = run<4, 2>(a, rows, wide, ty, s);
-    } else if (cols <= 512) {
-      rc = run<4, 4>(a, rows, wide, ty, s);
-    } else {
-      rc = run<4, 8>(a, rows, wide, ty, s);
-    }
+  if (vec && cg % 4 == 0) {
+    rc = run_width<4, true>(a, rows, cols, ty, s);
+  } else if (vec) {
+    rc = run_width<4, false>(a, rows, cols, ty, s);
   } else {
-    if (cols <= 128) {
-      rc = run<1, 4>(a, rows, wide, ty, s);
-    } else if (cols <= 512) {
-      rc = run<1, 16>(a, rows, wide, ty, s);
-    } else {
-      rc = run<1, 32>(a, rows, wide, ty, s);
-    }
+    rc = run_width<1, true>(a, rows, cols, ty, s);
   }
   if (rc == GNN_OK) clear_error();
   return rc;

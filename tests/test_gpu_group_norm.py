@@ -124,6 +124,46 @@ def test_many_random_graphs():
     _run(20000, 40, 5, ptr, "silu", seed=3)
 
 
+def _check_wide(n, c, groups, ptr, seed):
+    """The same bounds on the GPU, for row counts whose windows hold several long graphs."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(n, c, device=DEV, generator=g) + 2
+    out = torch.full_like(x, 7.0)
+    M.group_norm_forward_(x, groups, None, None, out, graph_ptr=ptr)
+    ptr = ptr.long()
+    seg = torch.searchsorted(ptr, torch.arange(n, device=DEV), right=True) - 1
+    inside = (seg >= 0) & (seg < len(ptr) - 1)
+    seg = seg.clamp(0, len(ptr) - 2)
+    v = x.double().view(n, groups, -1)
+    count = (ptr.diff().clamp(min=1) * (c // groups)).double()[:, None]
+    zero = torch.zeros(len(ptr) - 1, groups, dtype=torch.float64, device=DEV)
+    mean = zero.index_add(0, seg[inside], v.sum(2)[inside]) / count
+    d = v - mean[seg][:, :, None]
+    sd = (zero.index_add(0, seg[inside], d.square().sum(2)[inside]) / count + EPS).sqrt()[seg][:, :, None]
+    z = d / sd
+    biggest = float(x.abs().max())
+    bound = 24 * U * biggest / sd * (1 + z.abs()) + 28 * U * z.abs()
+    err = (out.double().view(n, groups, -1) - z).abs()
+    assert bool((err <= bound)[inside].all())
+    assert bool((out[~inside] == 7.0).all())
+
+
+@pytest.mark.parametrize("rows,graphs", [(200_003, 8192), (300_000, 3000), (400_000, 1500), (160_000, 100_000),
+                                         (1_000_000, 40)])
+def test_batches_of_many_rows(rows, graphs):
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    end = rows - rows // 50
+    cuts = torch.randint(0, end + 1, (graphs - 1,), device=DEV, generator=g).sort().values
+    ends = torch.tensor([0, end], device=DEV)
+    _check_wide(rows, 36, 4, torch.cat([ends[:1], cuts, ends[1:]]).to(torch.int32), rows)
+
+
+@pytest.mark.parametrize("length", [64, 65, 100, 128, 256, 257])
+def test_equal_graphs(length):
+    n = 1600 * length
+    _check_wide(n, 8, 2, torch.arange(0, n + 1, length, device=DEV), length)
+
+
 @pytest.mark.parametrize("ptr", [None, [0, 300]])
 def test_in_place(ptr):
     _run(300, 64, 4, ptr, "relu", inplace=True)
