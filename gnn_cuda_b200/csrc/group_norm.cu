@@ -253,17 +253,14 @@ __device__ __forceinline__ void load_affine(const NormArgs& a, const Tile<CH, NV
 }
 
 // blocks per SM that the registers have to allow
-#ifndef NB
-#define NB 3
-#endif
 template <int CH, int NV>
 constexpr int min_blocks() {
-  return CH * NV <= 4 ? NB : (CH * NV <= 8 ? 2 : 1);
+  return CH * NV <= 4 ? 3 : (CH * NV <= 8 ? 2 : 1);
 }
 
 // ---- each node on its own: one warp per row, R rows in flight ----------------
 template <int CH, int NV, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, min_blocks<CH, NV>()) norm_rows_kernel(NormArgs a) {
+__global__ void __launch_bounds__(kThreads, CH * NV <= 8 ? 4 : 1) norm_rows_kernel(NormArgs a) {
   constexpr int R = NV * CH <= 4 ? 4 : (NV * CH <= 8 ? 2 : 1);
   constexpr int E = WHOLE ? 1 : CH;
   extern __shared__ float scratch[];
@@ -314,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, min_blocks<CH, NV>()) norm_rows_kern
       for (int j = 0; j < NV; ++j) {
         if (t.live(j)) {
 #pragma unroll
-          for (int e = 0; e < E; ++e) q[j][e] = __frcp_rn(__fsqrt_rn(fmaf(q[j][e], inv, a.eps)));
+          for (int e = 0; e < E; ++e) q[j][e] = rsqrtf(fmaf(q[j][e], inv, a.eps));
 #pragma unroll
           for (int e = 0; e < CH; ++e) v[i][j][e] = fmaf(v[i][j][e] * q[j][e % E], w[j][e], b[j][e]);
         }
@@ -359,27 +356,56 @@ struct Team {
   // every size-th of `rows` rows
   __device__ __forceinline__ int count(int rows) const { return size == 1 ? rows : (rows + kWarps - 1) / kWarps; }
 
-  // rows first + size u of [first, end), as many as there are
-  __device__ __forceinline__ int load(const NormArgs& a, int64_t first, int64_t end) {
-    const int cnt = first < end ? min(U, count(static_cast<int>(end - first))) : 0;
+  // `cnt` rows (U of them where FULL), `step` floats apart, the first at p
+  template <bool FULL>
+  __device__ __forceinline__ void load(const float* p, int64_t step, int cnt) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (u < cnt && t.live(j)) {
-          load_chunk<CH>(a.x + (first + u * size) * a.c + t.channel(j), v[u][j]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < CH; ++e) v[u][j][e] = 0.0f;
-        }
+        if ((FULL || u < cnt) && t.live(j)) load_chunk<CH>(p + u * step + 32 * CH * j, v[u][j]);
       }
     }
-    return cnt;
   }
 
-  // (mean, M2) of the groups over rows [beg, end), the same in every warp; one batch of
-  // rows is left in v
-  __device__ __forceinline__ void stats(const NormArgs& a, int64_t beg, int64_t end, float (&mean)[NV][E],
+  // folds the rows in v into the running (m, s) of n rows a channel
+  template <bool FULL>
+  __device__ __forceinline__ void fold(int cnt, float& n, float (&m)[NV][CH], float (&s)[NV][CH]) {
+    const float cf = FULL ? static_cast<float>(U) : static_cast<float>(cnt);
+    const float icf = FULL ? 1.0f / U : __fdividef(1.0f, cf);
+    const float nn = n + cf;
+    const float share = __fdividef(cf, nn);
+    const float both = n * share;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (!t.live(j)) continue;
+#pragma unroll
+      for (int e = 0; e < CH; ++e) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (FULL || u < cnt) sum += v[u][j][e];
+        }
+        const float mb = sum * icf;
+        float dev = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (FULL || u < cnt) {
+            const float d = v[u][j][e] - mb;
+            dev = fmaf(d, d, dev);
+          }
+        }
+        const float d = mb - m[j][e];
+        m[j][e] = fmaf(d, share, m[j][e]);
+        s[j][e] += fmaf(d * d, both, dev);
+      }
+    }
+    n = nn;
+  }
+
+  // (mean, M2) of the groups over `rows` rows from row beg, the same in every warp; the
+  // last batch of rows is left in v
+  __device__ __forceinline__ void stats(const NormArgs& a, int64_t beg, int rows, float (&mean)[NV][E],
                                         float (&m2)[NV][E]) {
     float m[NV][CH], s[NV][CH];
 #pragma unroll
@@ -388,36 +414,16 @@ struct Team {
       for (int e = 0; e < CH; ++e) m[j][e] = s[j][e] = 0.0f;
     }
     float n = 0.0f;
-    for (int64_t r = beg; r < end; r += keep()) {
-      const int cnt = load(a, r + warp, end);
-      if (cnt == 0) break;
-      const float cf = static_cast<float>(cnt);
-      const float icf = __frcp_rn(cf);
-      const float nn = n + cf;
-      const float share = __fdividef(cf, nn);
-      const float both = n * share;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-#pragma unroll
-        for (int e = 0; e < CH; ++e) {
-          float sum = 0.0f;
-#pragma unroll
-          for (int u = 0; u < U; ++u) sum += v[u][j][e];
-          const float mb = sum * icf;
-          float dev = 0.0f;
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            if (u < cnt) {
-              const float d = v[u][j][e] - mb;
-              dev = fmaf(d, d, dev);
-            }
-          }
-          const float d = mb - m[j][e];
-          m[j][e] = fmaf(d, share, m[j][e]);
-          s[j][e] += fmaf(d * d, both, dev);
-        }
-      }
-      n = nn;
+    const int64_t step = static_cast<int64_t>(size) * a.c;
+    const float* p = a.x + (beg + warp) * a.c + t.channel(0);
+    int left = rows > warp ? count(rows - warp) : 0;
+    for (; left >= U; left -= U, p += U * step) {
+      load<true>(p, step, U);
+      fold<true>(U, n, m, s);
+    }
+    if (left > 0) {
+      load<false>(p, step, left);
+      fold<false>(left, n, m, s);
     }
     // the channels of a group: n values each
     const float icg = 1.0f / static_cast<float>(a.cg);
@@ -460,7 +466,6 @@ struct Team {
       }
     }
     __syncthreads();
-    const int64_t rows = end - beg;
     const float inv = 1.0f / static_cast<float>(rows);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -487,25 +492,54 @@ struct Team {
     }
   }
 
-  // normalises and stores the batch in v: rows first + 8 u
-  __device__ __forceinline__ void put(const NormArgs& a, int64_t first, int cnt, const float (&mean)[NV][E],
-                                      const float (&rstd)[NV][E], const float (&w)[NV][CH],
-                                      const float (&b)[NV][CH]) {
-with_activation(a.act, [&](auto act) {
+  // act(v * scale + shift) of the batch in v, stored at q, q + step, ...
+  template <int ACT, bool FULL>
+  __device__ __forceinline__ void put(float* q, int64_t step, int cnt, const float (&scale)[NV][CH],
+                                      const float (&shift)[NV][CH]) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (u >= cnt) break;
+    for (int u = 0; u < U; ++u) {
+      if (!FULL && u >= cnt) break;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          if (t.live(j)) {
+      for (int j = 0; j < NV; ++j) {
+        if (t.live(j)) {
 #pragma unroll
-            for (int e = 0; e < CH; ++e) {
-              v[u][j][e] = activate<decltype(act)::value>(
-                  fmaf((v[u][j][e] - mean[j][e % E]) * rstd[j][e % E], w[j][e], b[j][e]));
-            }
-            store_chunk<CH>(a.out + (first + u * size) * a.c + t.channel(j), v[u][j]);
-          }
+          for (int e = 0; e < CH; ++e) v[u][j][e] = activate<ACT>(fmaf(v[u][j][e], scale[j][e], shift[j][e]));
+          store_chunk<CH>(q + u * step + 32 * CH * j, v[u][j]);
         }
+      }
+    }
+  }
+
+  // Normalises `rows` rows from row beg, which are still in v where `kept`. mean and the
+  // affine part are folded into one multiply and add: the shift b - mean * scale is
+  // rounded once, an error like that of the 32-bit mean itself.
+  __device__ __forceinline__ void apply(const NormArgs& a, int64_t beg, int rows, bool kept, const float (&mean)[NV][E],
+                                        const float (&rstd)[NV][E], const float (&w)[NV][CH],
+                                        const float (&b)[NV][CH]) {
+    float scale[NV][CH], shift[NV][CH];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < CH; ++e) {
+        scale[j][e] = rstd[j][e % E] * w[j][e];
+        shift[j][e] = fmaf(-mean[j][e % E], scale[j][e], b[j][e]);
+      }
+    }
+    const int64_t step = static_cast<int64_t>(size) * a.c;
+    const int64_t at = (beg + warp) * a.c + t.channel(0);
+    const int mine = rows > warp ? count(rows - warp) : 0;
+    with_activation(a.act, [&](auto act) {
+      constexpr int ACT = decltype(act)::value;
+      const float* p = a.x + at;
+      float* q = a.out + at;
+      int left = mine;
+      for (; left >= U; left -= U, p += U * step, q += U * step) {
+        if (!kept) load<true>(p, step, U);
+        put<ACT, true>(q, step, U, scale, shift);
+      }
+      if (left > 0) {
+        if (!kept) load<false>(p, step, left);
+        put<ACT, false>(q, step, left, scale, shift);
       }
     });
   }
@@ -568,20 +602,15 @@ __global__ void __launch_bounds__(kThreads, min_blocks<CH, NV>()) norm_windows_k
   float w[NV][CH], b[NV][CH];
   load_affine(a, team.t, w, b);
   float mean[NV][E], m2[NV][E];
-  // normalises rows [s, e), whose statistics are (mean, m2)
-  auto finish = [&](int64_t s, int64_t e) {
-    const int rows = static_cast<int>(e - s);
+  // normalises `rows` rows from row s, whose statistics are (mean, m2)
+  auto finish = [&](int64_t s, int rows) {
     const float inv = 1.0f / (static_cast<float>(rows) * static_cast<float>(a.cg));
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
 #pragma unroll
-      for (int k = 0; k < E; ++k) m2[j][k] = __frcp_rn(__fsqrt_rn(fmaf(m2[j][k], inv, a.eps)));
+      for (int k = 0; k < E; ++k) m2[j][k] = rsqrtf(fmaf(m2[j][k], inv, a.eps));
     }
-    const bool kept = rows <= team.keep();  // they are still in registers
-    for (int64_t r = s + team.warp; r < e; r += team.keep()) {
-      const int cnt = kept ? team.count(static_cast<int>(e - r)) : team.load(a, r, e);
-      team.put(a, r, cnt, mean, m2, w, b);
-    }
+    team.apply(a, s, rows, rows <= team.keep(), mean, m2, w, b);
   };
   // Several short graphs: each warp takes one after the other by itself. Few: all
   // warps work on each.
@@ -598,18 +627,19 @@ __global__ void __launch_bounds__(kThreads, min_blocks<CH, NV>()) norm_windows_k
     }
     if (i >= shorts) break;
     const int item = list.item[i];
-    const int64_t s = r0 + (item >> 8), e = s + (item & 0xff);
-    team.stats(a, s, e, mean, m2);
-    finish(s, e);
+    const int64_t s = r0 + (item >> 8);
+    team.stats(a, s, item & 0xff, mean, m2);
+    finish(s, item & 0xff);
   }
   team.size = kWarps;
   team.warp = me;
   const int longs = min(list.longs, kMaxLongs);
   for (int i = 0; i < longs; ++i) {
     const int64_t s = list.begin[i], e = list.end[i];
-    team.stats(a, max(s, r0), min(e, r1), mean, m2);
+    const int64_t beg = max(s, r0);
+    team.stats(a, beg, static_cast<int>(min(e, r1) - beg), mean, m2);
     if (!is_split(a, s, e)) {
-      finish(s, e);
+      finish(s, static_cast<int>(e - s));
     } else if (me == 0) {
       float2* slot = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (s >= r0 ? 1 : 0)) * a.groups + team.t.g0;
 #pragma unroll
@@ -739,10 +769,8 @@ __global__ void __launch_bounds__(kThreads, min_blocks<CH, NV>()) norm_apply_ker
         rstd[j][k] = f.y;
       }
     }
-    const int64_t beg = max(s, r0), end = min(list.end[i], r1);
-    for (int64_t r = beg + team.warp; r < end; r += team.keep()) {
-      team.put(a, r, team.load(a, r, end), mean, rstd, w, b);
-    }
+    const int64_t beg = max(s, r0);
+    team.apply(a, beg, static_cast<int>(min(list.end[i], r1) - beg), false, mean, rstd, w, b);
   }
 }
 
