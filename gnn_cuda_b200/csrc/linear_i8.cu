@@ -56,7 +56,6 @@ struct I8Params {
   int64_t m_tiles;
   int n_tiles;
   int k_slices;
-  int stages;
   const float* x_scale;
   const float* w_scale;
   const float* bias;
@@ -91,29 +90,42 @@ __device__ __forceinline__ bool all_of_barrier(int threads, bool v) {
   return r != 0;
 }
 
-template <int BN, bool OUT8>
-constexpr int epilogue_warps() {
-  return OUT8 ? 8 : 4;
-}
+// One tile kernel: BN columns, 8-bit or fp32 output, EW epilogue warps.
+template <int BN, bool OUT8, int EW>
+struct Shape {
+  static constexpr int kHalves = EW / 4;  // epilogue warps per TMEM lane quarter
+  static constexpr int kCols = BN / kHalves >= 32 ? BN / kHalves : 32;  // columns per epilogue warp
+  // staging buffers per warp: with two, a block is written while the last one leaves
+  static constexpr int kBuffers = OUT8 || (BN == 256 && EW == 4) ? 1 : 2;
+  static constexpr size_t fixed() {
+    return 1024 /* alignment */ + EW * (kBuffers * kBlockBytes + kCols * 8) + (OUT8 ? kHalves * BM * 4 : 0) + 64;
+  }
+  static constexpr size_t bytes(int stages) { return fixed() + static_cast<size_t>(stages) * ((BM + BN) * KB + 16); }
+  static constexpr int stages() {
+    int s = kMaxStages;
+    while (bytes(s) > kSmemLimit) --s;
+    return s;
+  }
+};
 
-template <int BN, bool OUT8>
-__global__ void __launch_bounds__(64 + 32 * epilogue_warps<BN, OUT8>(), 1)
+template <int BN, bool OUT8, int EW>
+__global__ void __launch_bounds__(64 + 32 * EW, 1)
     linear_i8_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                      const __grid_constant__ CUtensorMap tmap_out, I8Params p) {
-  constexpr int EW = epilogue_warps<BN, OUT8>();
-  constexpr int HALVES = EW / 4;            // epilogue warps per TMEM lane quarter
-  constexpr int COLS = BN / HALVES >= 32 ? BN / HALVES : 32;  // columns per epilogue warp
+  using Sh = Shape<BN, OUT8, EW>;
+  constexpr int HALVES = Sh::kHalves;
+  constexpr int COLS = Sh::kCols;
+  constexpr int S = Sh::stages();
   constexpr uint32_t A_BYTES = BM * KB;
   constexpr uint32_t B_BYTES = BN * KB;
   constexpr uint32_t kTmemCols = 2 * BN;    // two accumulators; BN in {32, 64, 128, 256}
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int S = p.stages;
   uint8_t* sA = smem;
   uint8_t* sB = sA + S * A_BYTES;
-  uint8_t* sOut = sB + S * B_BYTES;                                      // EW x 4 KiB
-  float* sCol = reinterpret_cast<float*>(sOut + EW * kBlockBytes);      // EW x (32 scales + 32 biases)
-  float* sMax = sCol + EW * 64;                                         // OUT8: [HALVES][128]
+  uint8_t* sOut = sB + S * B_BYTES;                                   // staging of the epilogue warps
+  float* sCol = reinterpret_cast<float*>(sOut + EW * Sh::kBuffers * kBlockBytes);  // EW x (scales, biases)
+  float* sMax = sCol + EW * 2 * COLS;                                 // OUT8: [HALVES][128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sMax + (OUT8 ? HALVES * BM : 0));
   uint64_t* full = bars;
   uint64_t* empty = bars + S;
@@ -238,16 +250,31 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps<BN, OUT8>(), 1)
     const int half = ew / 4;
     const int cbeg = half * COLS;    // this warp's columns of the tile: [cbeg, cend)
     const int cend = cbeg + COLS <= BN ? cbeg + COLS : (cbeg < BN ? BN : cbeg);
-    uint8_t* staging = sOut + ew * kBlockBytes;
-    float* col = sCol + ew * 64;
+    uint8_t* staging = sOut + ew * (Sh::kBuffers * kBlockBytes);
+    float* scales = sCol + ew * 2 * COLS;  // of this warp's columns, read by all lanes as broadcasts
+    float* biases = scales + COLS;
     const bool has_bias = p.bias != nullptr;
     const bool relu = p.relu != 0;
     int acc = 0;
     uint32_t acc_phase = 0;
+    uint32_t blocks = 0;      // blocks staged so far
+    int64_t have_cols = -1;   // the column tile whose scales are there
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
       const int64_t row0 = (t / p.n_tiles) * BM + 32 * q;  // first row of this warp's lane quarter
-      const int64_t n0 = static_cast<int64_t>(t % p.n_tiles) * BN;
+      const int64_t n_tile = t % p.n_tiles;
+      const int64_t n0 = n_tile * BN;
       const float sx = row0 + lane < p.m ? __ldg(p.x_scale + row0 + lane) : 0.0f;
+      if (n_tile != have_cols) {
+        have_cols = n_tile;
+        __syncwarp();
+#pragma unroll
+        for (int c0 = 0; c0 < COLS; c0 += 32) {
+          const int64_t c = n0 + cbeg + c0 + lane;
+          scales[c0 + lane] = c < p.n ? __ldg(p.w_scale + c) : 0.0f;
+          biases[c0 + lane] = (has_bias && c < p.n) ? __ldg(p.bias + c) : 0.0f;
+        }
+        __syncwarp();
+      }
       // warp-uniform decision: the tcgen05.ld below is .sync.aligned. An 8-bit output's warps
       // meet at a barrier, so they decide together; that meeting also orders the last tile's
       // reads of sMax before this tile's writes.
@@ -259,69 +286,79 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps<BN, OUT8>(), 1)
       }
       tc_fence_after();
       const uint32_t taddr = tmem_base + static_cast<uint32_t>(acc * BN) + (static_cast<uint32_t>(32 * q) << 16);
-      // scales and biases of columns [c0, c0 + 32), read by the whole warp as broadcasts
-      auto load_cols = [&](int c0) {
-        __syncwarp();
-        const int64_t c = n0 + c0 + lane;
-        col[lane] = c < p.n ? __ldg(p.w_scale + c) : 0.0f;
-        col[32 + lane] = (has_bias && c < p.n) ? __ldg(p.bias + c) : 0.0f;
-        __syncwarp();
+      // y of columns [c0, c0 + 32) of this warp's share
+      auto transform = [&](int c0, uint32_t (&r)[32]) {
+        tmem_ld32(taddr + static_cast<uint32_t>(cbeg + c0), r);
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 sw = *reinterpret_cast<const float4*>(scales + c0 + j);
+          const float4 sb = *reinterpret_cast<const float4*>(biases + c0 + j);
+          r[j] = __float_as_uint(scaled(static_cast<int>(r[j]), sx, sw.x, sb.x, has_bias, relu));
+          r[j + 1] = __float_as_uint(scaled(static_cast<int>(r[j + 1]), sx, sw.y, sb.y, has_bias, relu));
+          r[j + 2] = __float_as_uint(scaled(static_cast<int>(r[j + 2]), sx, sw.z, sb.z, has_bias, relu));
+          r[j + 3] = __float_as_uint(scaled(static_cast<int>(r[j + 3]), sx, sw.w, sb.w, has_bias, relu));
+        }
       };
       if constexpr (!OUT8) {
         const bool has_rows = row0 < p.m;
 #pragma unroll 1
-        for (int c0 = cbeg; c0 < cend; c0 += 32) {
-          if (n0 + c0 >= p.n) break;
+        for (int c0 = 0; c0 < COLS && has_rows; c0 += 32) {
+          if (cbeg + c0 >= BN || n0 + cbeg + c0 >= p.n) break;
           uint32_t r[32];
-          tmem_ld32(taddr + static_cast<uint32_t>(c0), r);
-          load_cols(c0);
-          if (!has_rows) continue;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            r[j] = __float_as_uint(scaled(static_cast<int>(r[j]), sx, col[j], col[32 + j], has_bias, relu));
-          }
+          transform(c0, r);
+          uint8_t* buf = staging + (Sh::kBuffers == 2 ? (blocks & 1) * kBlockBytes : 0);
+          ++blocks;
           if (p.tma_store) {
-            if (lane == 0) bulk_wait_read_0();  // the last block has left the staging buffer
+            if (lane == 0) {  // the store that last used this buffer has read it
+              if constexpr (Sh::kBuffers == 2) {
+                bulk_wait_read_1();
+              } else {
+                bulk_wait_read_0();
+              }
+            }
             __syncwarp();
           }
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
-            *reinterpret_cast<uint4*>(staging + lane * 128 + ((((j >> 2) ^ (lane & 7))) << 4)) =
+            *reinterpret_cast<uint4*>(buf + lane * 128 + ((((j >> 2) ^ (lane & 7))) << 4)) =
                 make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
           }
           if (p.tma_store) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-              tma_store_2d(&tmap_out, staging, static_cast<int>(n0 + c0), static_cast<int>(row0));
+              tma_store_2d(&tmap_out, buf, static_cast<int>(n0 + cbeg + c0), static_cast<int>(row0));
               bulk_commit();
             }
           } else {
             __syncwarp();
-            const int64_t c = n0 + c0 + lane;
+            const int64_t c = n0 + cbeg + c0 + lane;
             const int rows = static_cast<int>(p.m - row0 < 32 ? p.m - row0 : 32);
             if (c < p.n) {
+              float* dst = p.out + row0 * p.ldo + c;
+#pragma unroll 8
               for (int j = 0; j < rows; ++j) {
-                p.out[(row0 + j) * p.ldo + c] = *reinterpret_cast<const float*>(
-                    staging + j * 128 + (((lane >> 2) ^ (j & 7)) << 4) + ((lane & 3) << 2));
+                dst[j * p.ldo] = *reinterpret_cast<const float*>(buf + j * 128 + (((lane >> 2) ^ (j & 7)) << 4) +
+                                                                ((lane & 3) << 2));
               }
             }
             __syncwarp();
           }
         }
       } else {
+        // one tile holds whole rows; a lane keeps its row's values in registers between
+        // the largest of them and the rounding
+        uint32_t r[COLS / 32][32];
         float amax = 0.0f;
-#pragma unroll 1
-        for (int c0 = cbeg; c0 < cend; c0 += 32) {
-          if (c0 >= p.n) break;
-          uint32_t r[32];
-          tmem_ld32(taddr + static_cast<uint32_t>(c0), r);
-          load_cols(c0);
-          const int live = static_cast<int>(p.n - c0 < 32 ? p.n - c0 : 32);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float y = scaled(static_cast<int>(r[j]), sx, col[j], col[32 + j], has_bias, relu);
-            if (j < live) amax = max_abs_nan(amax, y);
+        for (int b = 0; b < COLS / 32; ++b) {
+          if (cbeg + b * 32 < BN) {
+            transform(b * 32, r[b]);  // columns past n have scale and bias 0
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (cbeg + b * 32 + j >= p.n) r[b][j] = 0;  // 0 * an infinite or NaN row scale
+              amax = max_abs_nan(amax, __uint_as_float(r[b][j]));
+            }
           }
         }
         sMax[half * BM + 32 * q + lane] = amax;
@@ -330,29 +367,23 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps<BN, OUT8>(), 1)
         for (int h = 0; h < HALVES; ++h) amax = max_abs_nan(amax, sMax[h * BM + 32 * q + lane]);
         const RowQuant rq = row_quant(amax);
         if (half == 0 && row0 + lane < p.m) p.out_scale[row0 + lane] = rq.s;
-#pragma unroll 1
-        for (int c0 = cbeg; c0 < cend; c0 += 32) {
-          if (c0 >= p.n) break;
-          uint32_t r[32];
-          tmem_ld32(taddr + static_cast<uint32_t>(c0), r);
-          load_cols(c0);
-          // 32 columns are 32 bytes: two 16-byte chunks of this row's up to 128 staged bytes
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t b[4];
+        for (int b = 0; b < COLS / 32; ++b) {
+          if (cbeg + b * 32 < BN) {
+            // 32 columns are 32 bytes: two 16-byte chunks of this row's up to 128 staged bytes
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float y[4];
+            for (int h = 0; h < 2; ++h) {
+              uint32_t w[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int j = h * 16 + i * 4 + e;
-                y[e] = scaled(static_cast<int>(r[j]), sx, col[j], col[32 + j], has_bias, relu);
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t* y = &r[b][h * 16 + i * 4];
+                w[i] = quant4(rq, __uint_as_float(y[0]), __uint_as_float(y[1]), __uint_as_float(y[2]),
+                              __uint_as_float(y[3]));
               }
-              b[i] = quant4(rq, y[0], y[1], y[2], y[3]);
+              const int chunk = b * 2 + h;
+              *reinterpret_cast<uint4*>(staging + lane * 128 + ((chunk ^ (lane & 7)) << 4)) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
             }
-            const int chunk = (c0 - cbeg) / 16 + h;
-            *reinterpret_cast<uint4*>(staging + lane * 128 + ((chunk ^ (lane & 7)) << 4)) =
-                make_uint4(b[0], b[1], b[2], b[3]);
           }
         }
         __syncwarp();
@@ -372,8 +403,8 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps<BN, OUT8>(), 1)
             } else {
               const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (int b = 0; b < 16; ++b) {
-                if (b < bytes) dst[b] = static_cast<int8_t>((w[b >> 2] >> (8 * (b & 3))) & 0xffu);
+              for (int i = 0; i < 16; ++i) {
+                if (i < bytes) dst[i] = static_cast<int8_t>((w[i >> 2] >> (8 * (i & 3))) & 0xffu);
               }
             }
           }
@@ -502,13 +533,6 @@ int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 bool aligned_rows(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0; }
 
-template <int BN, bool OUT8>
-size_t smem_for(int stages) {
-  constexpr int EW = epilogue_warps<BN, OUT8>();
-  return 1024 + static_cast<size_t>(stages) * (BM + BN) * KB + EW * (kBlockBytes + 256) + (OUT8 ? EW / 4 * BM * 4 : 0) +
-         (2 * stages + 5) * 8 + 16;
-}
-
 int encode_rows(CUtensorMap* map, const int8_t* p, int64_t rows, int64_t k, int64_t ld, int box_rows) {
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
@@ -521,7 +545,7 @@ int encode_rows(CUtensorMap* map, const int8_t* p, int64_t rows, int64_t k, int6
   return GNN_OK;
 }
 
-template <int BN, bool OUT8>
+template <int BN, bool OUT8, int EW>
 int launch_bn(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int64_t k, I8Params p, cudaStream_t stream) {
   CUtensorMap tx{}, tw{}, to{};
   int rc = encode_rows(&tx, x, p.m, k, ldx, BM);
@@ -540,10 +564,9 @@ int launch_bn(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int64_
   p.m_tiles = (p.m + BM - 1) / BM;
   p.n_tiles = static_cast<int>((p.n + BN - 1) / BN);
   p.k_slices = static_cast<int>((k + KB - 1) / KB);
-  int stages = kMaxStages;
-  while (smem_for<BN, OUT8>(stages) > kSmemLimit) --stages;
-  p.stages = stages;
-  const size_t smem = smem_for<BN, OUT8>(stages);
+  constexpr int stages = Shape<BN, OUT8, EW>::stages();
+  constexpr size_t smem = Shape<BN, OUT8, EW>::bytes(stages);
+  static_assert(stages >= 2, "at least two stages have to fit");
   // the opt-in is a per-device function attribute
   static bool configured[64] = {};
   static std::mutex mu;
@@ -552,14 +575,14 @@ int launch_bn(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int64_
   {
     std::lock_guard<std::mutex> lock(mu);
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-      GNN_CUDA_TRY(cudaFuncSetAttribute(linear_i8_kernel<BN, OUT8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      GNN_CUDA_TRY(cudaFuncSetAttribute(linear_i8_kernel<BN, OUT8, EW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         static_cast<int>(smem)),
                    "linear_i8_kernel: shared memory opt-in");
       if (dev >= 0 && dev < 64) configured[dev] = true;
     }
   }
   const int64_t ctas = std::min<int64_t>(p.m_tiles * p.n_tiles, sm_count());
-  linear_i8_kernel<BN, OUT8><<<static_cast<unsigned>(ctas), 64 + 32 * epilogue_warps<BN, OUT8>(), smem, stream>>>(
+  linear_i8_kernel<BN, OUT8, EW><<<static_cast<unsigned>(ctas), 64 + 32 * EW, smem, stream>>>(
       tx, tw, to, p);
   GNN_LAUNCH_CHECK("linear_i8_kernel launch");
   return GNN_OK;
@@ -568,10 +591,14 @@ int launch_bn(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int64_
 template <bool OUT8>
 int launch(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int64_t k, const I8Params& p,
            cudaStream_t stream) {
-  if (p.n <= 32) return launch_bn<32, OUT8>(x, ldx, w, ldw, k, p, stream);
-  if (p.n <= 64) return launch_bn<64, OUT8>(x, ldx, w, ldw, k, p, stream);
-  if (p.n <= 128) return launch_bn<128, OUT8>(x, ldx, w, ldw, k, p, stream);
-  return launch_bn<256, OUT8>(x, ldx, w, ldw, k, p, stream);
+  if (p.n <= 32) return launch_bn<32, OUT8, 8>(x, ldx, w, ldw, k, p, stream);
+  if (p.n <= 64) return launch_bn<64, OUT8, 8>(x, ldx, w, ldw, k, p, stream);
+  if (p.n <= 128) return launch_bn<128, OUT8, 8>(x, ldx, w, ldw, k, p, stream);
+  if constexpr (!OUT8) {
+    // Long K: the MMAs are the bottleneck, and a fourth stage is worth more than a faster epilogue.
+    if (k >= 1024) return launch_bn<256, OUT8, 4>(x, ldx, w, ldw, k, p, stream);
+  }
+  return launch_bn<256, OUT8, 8>(x, ldx, w, ldw, k, p, stream);
 }
 
 // Whether the few-rows kernel takes the call: fp32 output, aligned w, rows that fit.
