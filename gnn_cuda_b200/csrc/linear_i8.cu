@@ -68,13 +68,13 @@ struct I8Params {
   int vec_store;     // 8-bit output rows are 16-byte aligned
 };
 
-// y of one element, rounded after each step
-__device__ __forceinline__ float scaled(int acc, float sx, float sw, float b, bool has_bias, bool relu) {
-  float y = __fmul_rn(__fmul_rn(__int2float_rn(acc), sx), sw);
-  if (has_bias) y = __fadd_rn(y, b);
-  if (relu && y < 0.0f) y = 0.0f;
-  return y;
+// y of one element, rounded after each step. Without a bias b is -0, which adds nothing
+// to any value; without ReLU `floor` is minus infinity, below which nothing lies.
+__device__ __forceinline__ float scaled(int acc, float sx, float sw, float b, float floor) {
+  const float y = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(acc), sx), sw), b);
+  return y < floor ? 0.0f : y;
 }
+__device__ __forceinline__ float floor_of(int relu) { return relu ? 0.0f : __int_as_float(0xff800000); }
 
 // Barrier 1 over `threads` threads; true where all of them came with true.
 __device__ __forceinline__ bool all_of_barrier(int threads, bool v) {
@@ -96,7 +96,7 @@ struct Shape {
   static constexpr int kHalves = EW / 4;  // epilogue warps per TMEM lane quarter
   static constexpr int kCols = BN / kHalves >= 32 ? BN / kHalves : 32;  // columns per epilogue warp
   // staging buffers per warp: with two, a block is written while the last one leaves
-  static constexpr int kBuffers = OUT8 || (BN == 256 && EW == 4) ? 1 : 2;
+  static constexpr int kBuffers = OUT8 || EW == 16 || (BN == 256 && EW == 4) ? 1 : 2;
   static constexpr size_t fixed() {
     return 1024 /* alignment */ + EW * (kBuffers * kBlockBytes + kCols * 8) + (OUT8 ? kHalves * BM * 4 : 0) + 64;
   }
@@ -253,8 +253,7 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
     uint8_t* staging = sOut + ew * (Sh::kBuffers * kBlockBytes);
     float* scales = sCol + ew * 2 * COLS;  // of this warp's columns, read by all lanes as broadcasts
     float* biases = scales + COLS;
-    const bool has_bias = p.bias != nullptr;
-    const bool relu = p.relu != 0;
+    const float floor = floor_of(p.relu);
     int acc = 0;
     uint32_t acc_phase = 0;
     uint32_t blocks = 0;      // blocks staged so far
@@ -271,7 +270,7 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
         for (int c0 = 0; c0 < COLS; c0 += 32) {
           const int64_t c = n0 + cbeg + c0 + lane;
           scales[c0 + lane] = c < p.n ? __ldg(p.w_scale + c) : 0.0f;
-          biases[c0 + lane] = (has_bias && c < p.n) ? __ldg(p.bias + c) : 0.0f;
+          biases[c0 + lane] = (p.bias != nullptr && c < p.n) ? __ldg(p.bias + c) : -0.0f;
         }
         __syncwarp();
       }
@@ -293,10 +292,10 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
         for (int j = 0; j < 32; j += 4) {
           const float4 sw = *reinterpret_cast<const float4*>(scales + c0 + j);
           const float4 sb = *reinterpret_cast<const float4*>(biases + c0 + j);
-          r[j] = __float_as_uint(scaled(static_cast<int>(r[j]), sx, sw.x, sb.x, has_bias, relu));
-          r[j + 1] = __float_as_uint(scaled(static_cast<int>(r[j + 1]), sx, sw.y, sb.y, has_bias, relu));
-          r[j + 2] = __float_as_uint(scaled(static_cast<int>(r[j + 2]), sx, sw.z, sb.z, has_bias, relu));
-          r[j + 3] = __float_as_uint(scaled(static_cast<int>(r[j + 3]), sx, sw.w, sb.w, has_bias, relu));
+          r[j] = __float_as_uint(scaled(static_cast<int>(r[j]), sx, sw.x, sb.x, floor));
+          r[j + 1] = __float_as_uint(scaled(static_cast<int>(r[j + 1]), sx, sw.y, sb.y, floor));
+          r[j + 2] = __float_as_uint(scaled(static_cast<int>(r[j + 2]), sx, sw.z, sb.z, floor));
+          r[j + 3] = __float_as_uint(scaled(static_cast<int>(r[j + 3]), sx, sw.w, sb.w, floor));
         }
       };
       if constexpr (!OUT8) {
@@ -520,7 +519,7 @@ __global__ void __launch_bounds__(kSmallThreads) linear_i8_small_kernel(SmallPar
 #pragma unroll
       for (int r = 1; r < MR; ++r) mine = lane == r ? acc[r] : mine;
       p.out[lane * p.ldo + j] = scaled(mine, sscale[lane], __ldg(p.w_scale + j),
-                                       p.bias != nullptr ? __ldg(p.bias + j) : 0.0f, p.bias != nullptr, p.relu != 0);
+                                       p.bias != nullptr ? __ldg(p.bias + j) : -0.0f, floor_of(p.relu));
     }
   }
 }
@@ -591,14 +590,14 @@ int launch_bn(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int64_
 template <bool OUT8>
 int launch(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int64_t k, const I8Params& p,
            cudaStream_t stream) {
-  if (p.n <= 32) return launch_bn<32, OUT8, 8>(x, ldx, w, ldw, k, p, stream);
+  if (p.n <= 32) return launch_bn<32, OUT8, 4>(x, ldx, w, ldw, k, p, stream);
   if (p.n <= 64) return launch_bn<64, OUT8, 8>(x, ldx, w, ldw, k, p, stream);
-  if (p.n <= 128) return launch_bn<128, OUT8, 8>(x, ldx, w, ldw, k, p, stream);
+  if (p.n <= 128) return launch_bn<128, OUT8, 16>(x, ldx, w, ldw, k, p, stream);
   if constexpr (!OUT8) {
     // Long K: the MMAs are the bottleneck, and a fourth stage is worth more than a faster epilogue.
     if (k >= 1024) return launch_bn<256, OUT8, 4>(x, ldx, w, ldw, k, p, stream);
   }
-  return launch_bn<256, OUT8, 8>(x, ldx, w, ldw, k, p, stream);
+  return launch_bn<256, OUT8, 16>(x, ldx, w, ldw, k, p, stream);
 }
 
 // Whether the few-rows kernel takes the call: fp32 output, aligned w, rows that fit.
