@@ -24,20 +24,21 @@ __device__ __forceinline__ float max_abs_nan(float a, float b) {
 
 struct RowQuant {
   float s;     // the scale that is stored
-  float sw;    // the scale times `lift`
+  float sw;    // the scale, times 2^80 where it is tiny, so that it is a normal number
   float inv;   // 1 / sw
   float half;  // sw / 2
-  float lift;  // power of two that keeps sw normal (1 unless the row is tiny)
-  bool none;   // q = 0 throughout
+  bool tiny;
+  uint32_t mask;  // 0 where q = 0 throughout
 };
 
 __device__ __forceinline__ RowQuant row_quant(float amax) {
   RowQuant r;
   const bool bad = !(amax < __int_as_float(0x7f800000));  // infinity or NaN
   r.s = bad ? __int_as_float(0x7fffffff) : __fdiv_rn(amax, 127.0f);
-  r.none = bad || r.s == 0.0f;
-  r.lift = r.s < 0x1p-60f ? 0x1p80f : 1.0f;
-  r.sw = r.none ? 1.0f : r.s * r.lift;
+  const bool none = bad || r.s == 0.0f;
+  r.mask = none ? 0u : 0xffffffffu;
+  r.tiny = !none && r.s < 0x1p-60f;
+  r.sw = none ? 1.0f : (r.tiny ? r.s * 0x1p80f : r.s);
   r.inv = __frcp_rn(r.sw);
   r.half = 0.5f * r.sw;
   return r;
@@ -48,9 +49,9 @@ constexpr float kRoundMagic = 12582912.0f;  // 1.5 * 2^23: adding it leaves the 
 // Four values of a row as four bytes.
 __device__ __forceinline__ uint32_t quant4(const RowQuant& r, float a, float b, float c, float d) {
   float v[4] = {a, b, c, d};
-  if (r.lift != 1.0f) {
+  if (r.tiny) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= r.lift;
+    for (int i = 0; i < 4; ++i) v[i] *= 0x1p80f;
   }
   float t[4], e[4];
   bool near = false;
@@ -60,7 +61,7 @@ __device__ __forceinline__ uint32_t quant4(const RowQuant& r, float a, float b, 
     e[i] = __fmaf_rn(-__fsub_rn(t[i], kRoundMagic), r.sw, v[i]);  // exact residual
     near |= fabsf(e[i]) >= r.half;
   }
-  if (near || r.lift != 1.0f) {  // at or beyond a border: ties go to the even neighbour
+  if (near || r.tiny) {  // at or beyond a border: ties go to the even neighbour
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float f = fabsf(e[i]);
@@ -71,7 +72,7 @@ __device__ __forceinline__ uint32_t quant4(const RowQuant& r, float a, float b, 
   }
   const uint32_t lo = __byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040);
   const uint32_t hi = __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040);
-  return r.none ? 0u : __byte_perm(lo, hi, 0x5410);
+  return __byte_perm(lo, hi, 0x5410) & r.mask;
 }
 
 __device__ __forceinline__ int8_t quant1(const RowQuant& r, float a) {

@@ -90,6 +90,32 @@ __device__ __forceinline__ bool all_of_barrier(int threads, bool v) {
   return r != 0;
 }
 
+// This CTA's tiles, column tiles first: tile blockIdx.x, then every gridDim.x-th.
+struct Walk {
+  int m, n;            // row tile, column tile
+  int dm, dn, n_tiles;
+  int64_t left;
+  __device__ __forceinline__ Walk(const I8Params& p) {
+    n_tiles = p.n_tiles;
+    const int grid = static_cast<int>(gridDim.x), first = static_cast<int>(blockIdx.x);
+    m = first / n_tiles;
+    n = first - m * n_tiles;
+    dm = grid / n_tiles;
+    dn = grid - dm * n_tiles;
+    left = (p.m_tiles * n_tiles - first + grid - 1) / grid;
+  }
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  __device__ __forceinline__ void next() {
+    --left;
+    m += dm;
+    n += dn;
+    if (n >= n_tiles) {
+      n -= n_tiles;
+      ++m;
+    }
+  }
+};
+
 // One tile kernel: BN columns, 8-bit or fp32 output, EW epilogue warps.
 template <int BN, bool OUT8, int EW>
 struct Shape {
@@ -136,7 +162,7 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int64_t tiles = p.m_tiles * p.n_tiles;
+  Walk at(p);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -169,9 +195,9 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
       uint32_t phase = 0;
       int64_t issued = 0;
       bool ok = true;
-      for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const int row = static_cast<int>((t / p.n_tiles) * BM);
-        const int col = static_cast<int>(t % p.n_tiles) * BN;
+      for (; at.more() && ok; at.next()) {
+        const int row = at.m * BM;
+        const int col = at.n * BN;
         for (int ks = 0; ks < p.k_slices; ++ks) {
           if (!mbar_wait(&empty[stage], phase ^ 1)) {
             record_timeout(33);
@@ -209,7 +235,7 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
       uint32_t phase = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
-      for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (; at.more() && ok; at.next()) {
         if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1)) {
           record_timeout(34);
           break;
@@ -257,12 +283,19 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
     int acc = 0;
     uint32_t acc_phase = 0;
     uint32_t blocks = 0;      // blocks staged so far
-    int64_t have_cols = -1;   // the column tile whose scales are there
-    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-      const int64_t row0 = (t / p.n_tiles) * BM + 32 * q;  // first row of this warp's lane quarter
-      const int64_t n_tile = t % p.n_tiles;
-      const int64_t n0 = n_tile * BN;
-      const float sx = row0 + lane < p.m ? __ldg(p.x_scale + row0 + lane) : 0.0f;
+    int have_cols = -1;       // the column tile whose scales are there
+    auto load_scale = [&]() -> float {
+      const int64_t r = static_cast<int64_t>(at.m) * BM + 32 * q + lane;
+      return at.more() && r < p.m ? __ldg(p.x_scale + r) : 0.0f;
+    };
+    float sx_next = load_scale();
+    while (at.more()) {
+      const int64_t row0 = static_cast<int64_t>(at.m) * BM + 32 * q;  // first row of this warp's lane quarter
+      const int n_tile = at.n;
+      const int64_t n0 = static_cast<int64_t>(n_tile) * BN;
+      const float sx = sx_next;
+      at.next();
+      sx_next = load_scale();  // a tile ahead of its use
       if (n_tile != have_cols) {
         have_cols = n_tile;
         __syncwarp();
@@ -352,12 +385,14 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
 #pragma unroll
         for (int b = 0; b < COLS / 32; ++b) {
           if (cbeg + b * 32 < BN) {
-            transform(b * 32, r[b]);  // columns past n have scale and bias 0
+            transform(b * 32, r[b]);
+            if (p.n < BN) {  // columns past n are 0 * x_scale, which an infinite or NaN scale makes NaN
+              const int live = static_cast<int>(p.n) - cbeg - b * 32;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              if (cbeg + b * 32 + j >= p.n) r[b][j] = 0;  // 0 * an infinite or NaN row scale
-              amax = max_abs_nan(amax, __uint_as_float(r[b][j]));
+              for (int j = 0; j < 32; ++j) r[b][j] = j < live ? r[b][j] : 0u;
             }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) amax = max_abs_nan(amax, __uint_as_float(r[b][j]));
           }
         }
         sMax[half * BM + 32 * q + lane] = amax;
