@@ -4,6 +4,9 @@ Same flags, memory placement, UVM hints/prefetch, ``--ft_host_alloc`` device
 reserve and printed report as the reference. Per layer:
     agg = Â·x                    (spmm_gcn_forward_ / spmm_pyg_gcn_forward_)
     out = relu?(agg·W + b)       (linear_forward_: tcgen05 GEMM, bias+ReLU fused)
+With ``--features int8`` the layer inputs are held in 8-bit rows and both steps run on
+them (spmm_int8_forward_, linear_int8_forward_); with ``--norm`` the hidden layers'
+ReLU becomes a group norm with ReLU (group_norm_forward_).
 ReLU on every layer but the last. The reference ran GEMM and bias/ReLU as two
 launches and synchronised after every phase; here the phases only record
 CUDA events, so one forward is a single stream of launches.
@@ -33,6 +36,8 @@ from .allocator import (
     uses_cuda_memory_hints,
 )
 from .gcn_ops import spmm_gcn_forward_, stage_feature_rows_
+from .int8_ops import empty_rows, linear_int8_forward_, quantize_rows_, quantize_weight_, spmm_int8_forward_
+from .norm_ops import group_norm_forward_
 from .graph_utils import (
     apply_node_permutation,
     build_gcn_normalized_csr,
@@ -94,6 +99,31 @@ def _make_layer_state(in_dim, out_dim, *, num_nodes, device, weight_mode, activa
     return LayerState(w, b, agg, out)
 
 
+@dataclass
+class Int8LayerState:
+    """What a layer needs beside its LayerState when its input is held in 8 bits."""
+    x: torch.Tensor
+    x_scale: torch.Tensor
+    weight: torch.Tensor
+    weight_scale: torch.Tensor
+
+
+def _make_int8_state(layer: LayerState, *, num_nodes: int, device) -> Int8LayerState:
+    in_dim, out_dim = layer.weight.shape
+    st = Int8LayerState(empty_rows(num_nodes, in_dim, device), torch.empty(num_nodes, device=device),
+                        empty_rows(out_dim, in_dim, device), torch.empty(out_dim, device=device))
+    quantize_weight_(layer.weight, st.weight, st.weight_scale)
+    return st
+
+
+def _check_int8_args(args, place, device, spmm_mode: str) -> None:
+    if device.type != "cuda" or (place.adj, place.ft, place.weight, place.activation) != ("device",) * 4:
+        raise ValueError("--features int8 needs a CUDA device and device placement (--memory_mode device)")
+    if spmm_mode == "optimized" or bool(args.fuse_layers) or str(args.layer_order) == "transform_first":
+        raise ValueError("--features int8 aggregates first and works with neither --spmm_mode optimized nor "
+                         "--fuse_layers")
+
+
 def _resolve_preprocess_meta_path(mode: str, *, dataset: str, data_root: str) -> str | None:
     if mode == "none":
         return None
@@ -116,6 +146,13 @@ def build_parser():
     p.add_argument("--preprocess_meta", type=str, default="none", help=argparse.SUPPRESS)
     p.add_argument("--pretouch_passes", type=int, default=0, help=argparse.SUPPRESS)
     D.add_runtime_flags(p)
+    p.add_argument("--features", type=str, default="fp32", choices=["fp32", "int8"],
+                   help="int8: every layer's input held in signed 8-bit rows with one scale per node, aggregated and "
+                        "transformed on the 8-bit path (device placement only)")
+    p.add_argument("--norm", type=str, default="none", choices=["none", "node", "graph"],
+                   help="group norm with ReLU after every layer but the last, instead of ReLU alone: of each node on "
+                        "its own, or over all nodes of the graph")
+    p.add_argument("--norm_groups", type=int, default=8, help="channel groups of --norm")
     p.add_argument("--ft_host_alloc", type=float, default=0.0,
                    help="target percent of the feature matrix that should not fit in the remaining effective GPU memory")
     p.add_argument("--prefetch_pieces", type=int, default=0,
@@ -205,6 +242,15 @@ def run_gcn_inference(*, framework_label: str, select_device: Callable[[str], to
             torch.cuda.empty_cache()
             torch.cuda.synchronize(device)
 
+    norm, norm_groups = str(args.norm), int(args.norm_groups)
+    if norm != "none" and (norm_groups < 1 or int(args.hidden_dim) % norm_groups != 0):
+        raise ValueError("--norm_groups must divide the hidden dimension")
+    if norm != "none" and device.type != "cuda":
+        raise ValueError("--norm needs a CUDA device")
+    int8 = str(args.features) == "int8"
+    if int8:
+        _check_int8_args(args, place, device, spmm_mode)
+
     overlap_pieces = int(args.prefetch_pieces)
     if overlap_pieces < 0:
         raise ValueError("--prefetch_pieces expects a value >= 0")
@@ -277,6 +323,8 @@ def run_gcn_inference(*, framework_label: str, select_device: Callable[[str], to
         dims = D.layer_dims(int(features_cpu.size(1)), int(args.hidden_dim), int(args.out_dim), int(args.num_layers))
         plans = [_layer_plan(args, idx, i, o, device=device, impl=impl, optimized_first=optimized_active)
                  for idx, (i, o) in enumerate(dims)]
+        if int8:
+            plans = ["int8"] * len(dims)
         print(f"Layer plan: {', '.join(plans)}")
         layers = [_make_layer_state(i, o, num_nodes=int(num_nodes), device=device, weight_mode=place.weight,
                                     activation_mode=place.activation, cfg=cfg, plan=plan)
@@ -316,6 +364,11 @@ def run_gcn_inference(*, framework_label: str, select_device: Callable[[str], to
                                      nbytes=rs["prefetch"] if reserve_on else None)
             else:
                 prefetch_managed(features, location=cfg.prefetch_to, device=device)
+        int8_states = []
+        if int8:
+            int8_states = [_make_int8_state(layer, num_nodes=int(num_nodes), device=device) for layer in layers]
+            quantize_rows_(features, int8_states[0].x, int8_states[0].x_scale)
+        norm_ptr = torch.tensor([0, int(num_nodes)], device=device) if norm == "graph" else None
         if hot_cache is not None:
             stage_feature_rows_(features, hot_cache)
         if optimized_active:
@@ -368,7 +421,7 @@ def run_gcn_inference(*, framework_label: str, select_device: Callable[[str], to
                 if plans[idx] == "fused":
                     # aggregation and transform in one kernel: the layer's output directly
                     gcn_layer_forward_(row_ptr, col_ind, deg_inv_sqrt, x, layer.weight, layer.bias, layer.out_buffer,
-                                       relu=idx != len(layers) - 1)
+                                       relu=idx != len(layers) - 1 and norm == "none")
                 elif impl == "pyg_baseline":
                     spmm_pyg_gcn_forward_(row_ptr, col_ind, edge_weight, x, dst, spmm_mode=mode,
                                           optimized_backend=place.ft if first else "hmm",
@@ -381,7 +434,40 @@ def run_gcn_inference(*, framework_label: str, select_device: Callable[[str], to
                                       hot_feature_cache=hot_cache if first else None,
                                       hot_node_cutoff=hot_cutoff if first else 0)
 
+    def normalise(layer: LayerState) -> None:
+        with phases.measure("epilogue"):
+            group_norm_forward_(layer.out_buffer, norm_groups, None, None, layer.out_buffer, graph_ptr=norm_ptr,
+                                activation="relu")
+
+    def forward_int8() -> torch.Tensor:
+        """Every layer on 8-bit rows: aggregate to fp32, transform (its rows quantised on the way), and leave
+        the next layer's input in 8 bits, straight from the transform where no norm comes between."""
+        for idx, (layer, st) in enumerate(zip(layers, int8_states)):
+            last = idx == len(layers) - 1
+            tag = f"layer{idx + 1}"
+            with D.nvtx_range(nvtx, f"{tag}/aggregation"):
+                with phases.measure("spmm"):
+                    spmm_int8_forward_(row_ptr, col_ind, st.x, st.x_scale, layer.agg_buffer,
+                                       aggregation="weighted" if impl == "pyg_baseline" else "gcn",
+                                       deg_inv_sqrt=deg_inv_sqrt, edge_weight=edge_weight)
+            nxt = None if last else int8_states[idx + 1]
+            with D.nvtx_range(nvtx, f"{tag}/dense_update"):
+                with phases.measure("gemm"):
+                    if last or norm != "none":
+                        linear_int8_forward_(layer.agg_buffer, None, st.weight, st.weight_scale, layer.bias,
+                                             layer.out_buffer)
+                    else:
+                        linear_int8_forward_(layer.agg_buffer, None, st.weight, st.weight_scale, layer.bias, nxt.x,
+                                             relu=True, out_scale=nxt.x_scale)
+            if not last and norm != "none":
+                normalise(layer)
+                with phases.measure("gemm"):
+                    quantize_rows_(layer.out_buffer, nxt.x, nxt.x_scale)
+        return layers[-1].out_buffer
+
     def forward_once() -> torch.Tensor:
+        if int8:
+            return forward_int8()
         x = features
         for idx, layer in enumerate(layers):
             tag = f"layer{idx + 1}"
@@ -390,7 +476,7 @@ def run_gcn_inference(*, framework_label: str, select_device: Callable[[str], to
                 mode = "optimized"
             elif idx != 0 and mode == "optimized":
                 mode = "plain"
-            relu = idx != len(layers) - 1
+            relu = idx != len(layers) - 1 and norm == "none"
             src, dst = x, None
             if plans[idx] == "transform_first":
                 # A·(x·W): the narrower x·W rows are gathered; bias and ReLU after the aggregation
@@ -416,6 +502,8 @@ def run_gcn_inference(*, framework_label: str, select_device: Callable[[str], to
             elif plans[idx] == "transform_first":
                 with phases.measure("gemm"):
                     bias_relu_forward_(layer.out_buffer, layer.bias, relu)
+            if norm != "none" and idx != len(layers) - 1:
+                normalise(layer)
             x = layer.out_buffer
         return x
 
@@ -454,6 +542,10 @@ def run_gcn_inference(*, framework_label: str, select_device: Callable[[str], to
     print(f"Weight Memory Mode:\t{place.weight}")
     print(f"Activation Memory Mode:\t{place.activation}")
     print(f"GCN Kernel Impl:\t{impl}")
+    if int8:
+        print("Feature Rows:\tint8")
+    if norm != "none":
+        print(f"Norm:\t{norm} ({norm_groups} groups)")
     print(f"SpMM Mode:\t{spmm_mode}")
     print(f"Pre-touch Passes:\t{int(args.pretouch_passes)}")
     print(f"Feature Host Alloc Target (%):\t{ft_host_alloc:.3f}")
@@ -504,7 +596,9 @@ def run_gcn_inference(*, framework_label: str, select_device: Callable[[str], to
                                       int(features.data_ptr()) + features.numel() * features.element_size()),
                        spmm_avg_ns=phases.avg_ns("spmm", iters=int(args.iters)), iters=int(args.iters))
         capture.update(output=output.detach().cpu(), features=features.detach().cpu(), layers=layers,
-                       row_ptr=row_ptr.detach().cpu(), col_ind=col_ind.detach().cpu(), num_nodes=num_nodes)
+                       row_ptr=row_ptr.detach().cpu(), col_ind=col_ind.detach().cpu(), num_nodes=num_nodes,
+                       deg_inv_sqrt=None if deg_inv_sqrt is None else deg_inv_sqrt.detach().cpu(),
+                       edge_weight=None if edge_weight is None else edge_weight.detach().cpu())
     print(f"Output Sum:\t{float(output.sum().item()):.6f}")
     infer_avg_ns = elapsed * 1e9 / args.iters
     print(f"Infer (ns):\t{infer_avg_ns:.3f}")

@@ -85,3 +85,15 @@ def test_spmm_python_refusals():
     rp, ci = torch.zeros(5, dtype=torch.int32), torch.zeros(0, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="out must be CUDA"):
         I.spmm_int8_forward_(rp, ci, torch.zeros(4, 8, dtype=torch.int8), torch.ones(4), torch.zeros(4, 8))
+
+
+@pytest.mark.parametrize("argv,match", [
+    (["--features", "int8"], "needs a CUDA device and device placement"),
+    (["--norm", "node"], "needs a CUDA device"),
+    (["--norm", "graph", "--norm_groups", "3"], "must divide the hidden dimension"),
+])
+def test_driver_refusals(argv, match):
+    from gnn_cuda_b200.GNN_cuda_common import gcn_inference
+    with pytest.raises(ValueError, match=match):
+        gcn_inference.run_gcn_inference(framework_label="pyg", select_device=torch.device, load_graph_features=None,
+                                        load_kind="pyg", argv=["--device", "cpu", "--memory_mode", "device", *argv])
