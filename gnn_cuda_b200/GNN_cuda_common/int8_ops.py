@@ -20,6 +20,8 @@ graphs never share it.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _native as N
@@ -43,7 +45,8 @@ _I8, _F32 = torch.int8, torch.float32
 def _device_of(out: torch.Tensor, name: str = "out") -> int:
     """The output's device index; it is made current by _on() around the call."""
     index = out.get_device()
-    _check(index >= 0 and out.is_cuda, f"{name} must be CUDA")
+    if index < 0 or not out.is_cuda:
+        _check(False, f"{name} must be CUDA")
     return index
 
 
@@ -119,8 +122,17 @@ class _On:
             torch.cuda.set_device(self.old)
 
 
-def _scratch(nbytes: int, index: int) -> torch.Tensor | None:
-    return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index)) if nbytes else None
+def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor | None:
+    """Uninitialised bytes on the device of `like`, from the allocator's pool of the current stream."""
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+
+
+def _launch(index: int, call):
+    """call(stream) with the device made current."""
+    if _current_device is not None and _current_stream is not None and _current_device() == index:
+        return call(_current_stream(index))
+    with _On(index) as stream:
+        return call(stream)
 
 
 def quantize_rows_(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
@@ -160,6 +172,66 @@ def linear_int8_forward_(x: torch.Tensor, x_scale: torch.Tensor | None, weight: 
     quantised on the way). weight: int8 [n, k] with weight_scale [n]
     (``quantize_weight_``). out: float32 [m, n], or int8 [m, n] with out_scale [m]
     (quantised as ``quantize_rows_`` would quantise the float32 result)."""
+    m, k, n, ldx, ldw, ldo = (_linear_sizes_quick(x, x_scale, weight, weight_scale, bias, out, out_scale)
+                              or _linear_sizes(x, x_scale, weight, weight_scale, bias, out, out_scale))
+    xp, wp, op = x.data_ptr(), weight.data_ptr(), out.data_ptr()
+    x_type = N.GNN_ROWS_FP32 if x_scale is None else N.GNN_ROWS_INT8
+    out_type = N.GNN_ROWS_FP32 if out_scale is None else N.GNN_ROWS_INT8
+    lib = N.lib()
+    args = (xp, x_type, ldx, None if x_scale is None else x_scale.data_ptr(), wp, ldw, weight_scale.data_ptr(),
+            None if bias is None or bias.numel() == 0 else bias.data_ptr(), op, out_type, ldo,
+            None if out_scale is None else out_scale.data_ptr(), m, k, n, 1 if relu else 0)
+
+    def call(stream):
+        # Most calls on 8-bit rows need no scratch: the entry point says where one does, before it launches
+        # anything. fp32 rows need it but for the fewest.
+        rc = N.GNN_ERR_WORKSPACE
+        if x_scale is not None or m <= 8:
+            rc = lib.gnn_linear_int8_forward(*args, None, 0, stream)
+        if rc == N.GNN_ERR_WORKSPACE:
+            wsb = lib.gnn_linear_int8_workspace_bytes(xp, x_type, ldx, wp, ldw, out_type, m, k, n)
+            ws = _scratch(wsb, out)
+            rc = lib.gnn_linear_int8_forward(*args, None if ws is None else ws.data_ptr(), wsb, stream)
+        return rc
+
+    rc = _launch(out.get_device(), call)
+    if rc:
+        N.check(rc, "gnn_linear_int8_forward")
+
+
+def _vector_ok(t: torch.Tensor, length: int, index: int) -> bool:
+    return (t.dtype is _F32 and t.get_device() == index and t.shape == (length,)
+            and (length < 2 or t.stride(0) == 1))
+
+
+def _linear_sizes_quick(x, x_scale, weight, weight_scale, bias, out, out_scale):
+    """The sizes of a call with fp32 output that passes every check of _linear_sizes, found in fewer steps;
+    None where that is not plain."""
+    index = out.get_device()
+    if out_scale is not None or out.dtype is not _F32 or not out.is_contiguous() or not out.is_cuda:
+        return None
+    if x.dim() != 2 or weight.dim() != 2 or out.dim() != 2 or weight.dtype is not _I8:
+        return None
+    (m, k), (n, kw), (mo, no) = x.shape, weight.shape, out.shape
+    (ldx, sx), (ldw, sw) = x.stride(), weight.stride()
+    if (k != kw or m != mo or n != no or sx != 1 or sw != 1 or ldx < k or ldw < k or k < 1
+            or x.get_device() != index or weight.get_device() != index):
+        return None
+    if x.dtype is _I8:
+        if x_scale is None or not _vector_ok(x_scale, m, index):
+            return None
+    elif x.dtype is not _F32 or x_scale is not None or (ldx != k and m > 1):
+        return None
+    if not _vector_ok(weight_scale, n, index) or not (bias is None or _vector_ok(bias, n, index)):
+        return None
+    xp, op = x.data_ptr(), out.data_ptr()
+    if not (op + 4 * m * n <= xp or xp + m * ldx * x.element_size() <= op):
+        return None
+    return m, k, n, ldx, ldw, n
+
+
+def _linear_sizes(x, x_scale, weight, weight_scale, bias, out, out_scale) -> tuple[int, int, int, int, int, int]:
+    """The checks of linear_int8_forward_: (m, k, n, ldx, ldw, ldo)."""
     index = _device_of(out)
     ldw = _check_rows8("weight", weight, index)
     n, k = weight.shape
@@ -168,12 +240,11 @@ def linear_int8_forward_(x: torch.Tensor, x_scale: torch.Tensor | None, weight: 
         ldx = _check_rows8("x", x, index)
         _check(x_scale is not None, "x_scale is needed for int8 x")
         _check_vector("x_scale", x_scale, x.shape[0], index, "the number of rows")
-        x_type, xs_ptr = N.GNN_ROWS_INT8, x_scale.data_ptr()
     else:
         _check(x.dtype is _F32, "x must be int8 or float32")
         _check_f32("x", x, 2, index)
         _check(x_scale is None, "x_scale must be None for float32 x")
-        x_type, xs_ptr, ldx = N.GNN_ROWS_FP32, None, x.shape[1]
+        ldx = x.shape[1]
     m = x.shape[0]
     _check(k == x.shape[1], "Inner GEMM dimensions must match")
     _check(k >= 1, "x must have at least one column")
@@ -182,30 +253,21 @@ def linear_int8_forward_(x: torch.Tensor, x_scale: torch.Tensor | None, weight: 
         ldo = _check_rows8("out", out, index)
         _check(out_scale is not None, "out_scale is needed for int8 out")
         _check_vector("out_scale", out_scale, m, index, "the number of rows")
-        out_type, os_ptr = N.GNN_ROWS_INT8, out_scale.data_ptr()
     else:
         _check(out.dtype is _F32, "out must be int8 or float32")
         _check(out.is_contiguous(), "out must be contiguous")
         _check(out_scale is None, "out_scale must be None for float32 out")
-        out_type, os_ptr, ldo = N.GNN_ROWS_FP32, None, n
-    bias_ptr = None
+        ldo = n
     if bias is not None and bias.numel() != 0:
         _check_vector("bias", bias, n, index, "output feature dimension")
-        bias_ptr = bias.data_ptr()
-    xp, wp, op = x.data_ptr(), weight.data_ptr(), out.data_ptr()
-    _check_apart(out, op, ldo, x, xp, ldx)
-    lib = N.lib()
-    args = (xp, x_type, ldx, xs_ptr, wp, ldw, weight_scale.data_ptr(), bias_ptr, op, out_type, ldo, os_ptr, m, k, n,
-            1 if relu else 0)
-    with _On(index) as stream:
-        # most calls need no scratch: the entry point says where one does, before it launches anything
-        rc = lib.gnn_linear_int8_forward(*args, None, 0, stream)
-        if rc == N.GNN_ERR_WORKSPACE:
-            wsb = lib.gnn_linear_int8_workspace_bytes(xp, x_type, ldx, wp, ldw, out_type, m, k, n)
-            ws = _scratch(wsb, index)
-            rc = lib.gnn_linear_int8_forward(*args, ws.data_ptr(), wsb, stream)
-        if rc:
-            N.check(rc, "gnn_linear_int8_forward")
+    _check_apart(out, out.data_ptr(), ldo, x, x.data_ptr(), ldx)
+    return m, k, n, ldx, ldw, ldo
+
+
+@functools.lru_cache(maxsize=1024)
+def _spmm_workspace(index: int, n: int, nnz: int, f: int) -> int:
+    """A size by sizes: asked once for each (the device is current)."""
+    return N.lib().gnn_spmm_int8_workspace_bytes(n, nnz, f)
 
 
 _WEIGHTING = {"sum": N.GNN_WEIGHT_SUM, "mean": N.GNN_WEIGHT_MEAN, "gcn": N.GNN_WEIGHT_GCN,
@@ -228,8 +290,10 @@ def spmm_int8_forward_(row_ptr: torch.Tensor, col_ind: torch.Tensor, x: torch.Te
     _check(weighting is not None, "aggregation must be sum, mean, gcn or weighted")
     for name, t in (("row_ptr", row_ptr), ("col_ind", col_ind)):
         _same_device(name, t, index)
-        _check(t.is_contiguous(), f"{name} must be contiguous")
-        _check(t.dim() == 1, f"{name} must be rank-1")
+        if not t.is_contiguous():
+            _check(False, f"{name} must be contiguous")
+        if t.dim() != 1:
+            _check(False, f"{name} must be rank-1")
     row_type = _index_type(row_ptr)
     _check(col_ind.dtype is torch.int32, "col_ind must be int32")
     ldx = _check_rows8("x", x, index)
@@ -237,12 +301,14 @@ def spmm_int8_forward_(row_ptr: torch.Tensor, col_ind: torch.Tensor, x: torch.Te
     _check(x.shape == out.shape, "x and out must have the same shape")
     n, f = out.shape
     nnz = col_ind.shape[0]
-    _check_vector("x_scale", x_scale, n, index, "num_nodes")
+    if not _vector_ok(x_scale, n, index):
+        _check_vector("x_scale", x_scale, n, index, "num_nodes")
     _check(row_ptr.shape[0] == n + 1, "row_ptr length must be num_nodes + 1")
     dis_ptr = ew_ptr = None
     if aggregation == "gcn":
         _check(deg_inv_sqrt is not None, "deg_inv_sqrt is needed for gcn")
-        _check_vector("deg_inv_sqrt", deg_inv_sqrt, n, index, "num_nodes")
+        if not _vector_ok(deg_inv_sqrt, n, index):
+            _check_vector("deg_inv_sqrt", deg_inv_sqrt, n, index, "num_nodes")
         dis_ptr = deg_inv_sqrt.data_ptr()
     else:
         _check(deg_inv_sqrt is None, "deg_inv_sqrt is only for gcn")
@@ -254,11 +320,14 @@ def spmm_int8_forward_(row_ptr: torch.Tensor, col_ind: torch.Tensor, x: torch.Te
         _check(edge_weight is None, "edge_weight is only for weighted")
     xp, op = x.data_ptr(), out.data_ptr()
     _check_apart(out, op, f, x, xp, ldx)
-    lib = N.lib()
-    with _On(index) as stream:
-        wsb = lib.gnn_spmm_int8_workspace_bytes(n, nnz, f)
-        ws = _scratch(wsb, index)
-        N.check(lib.gnn_spmm_int8_forward(row_ptr.data_ptr(), row_type, col_ind.data_ptr(), weighting, dis_ptr, ew_ptr,
-                                          xp, ldx, x_scale.data_ptr(), op, n, nnz, f,
-                                          None if ws is None else ws.data_ptr(), wsb, stream),
-                "gnn_spmm_int8_forward")
+    args = (row_ptr.data_ptr(), row_type, col_ind.data_ptr(), weighting, dis_ptr, ew_ptr, xp, ldx, x_scale.data_ptr(),
+            op, n, nnz, f)
+
+    def call(stream):
+        wsb = _spmm_workspace(index, n, nnz, f)
+        ws = _scratch(wsb, out)
+        return N.lib().gnn_spmm_int8_forward(*args, None if ws is None else ws.data_ptr(), wsb, stream)
+
+    rc = _launch(index, call)
+    if rc:
+        N.check(rc, "gnn_spmm_int8_forward")
