@@ -252,12 +252,18 @@ __device__ __forceinline__ void load_affine(const NormArgs& a, const Tile<CH, NV
   }
 }
 
-// Blocks per SM that the registers have to allow. Measured on the ragged batch (200,003
-// rows, 8,192 graphs): 3 against 2 blocks 82 / 90 us where a chunk lies in one group
-// (C = 128), 113 / 101 us where it does not (C = 100), whose registers then spill.
+// Rows of a warp in flight, and blocks per SM that the registers have to allow. Measured
+// on the ragged batch (200,003 rows, 8,192 graphs): where a chunk lies in one group (C =
+// 128, no activation) 8 rows and 3 blocks 82 us, 4 rows and 3 blocks 89 us, 8 rows and 2
+// blocks 90 us; where it does not (C = 100, GELU), which takes more registers, 4 rows and
+// 3 blocks 119 us, 8 rows and 3 blocks (spilling) 165 us, 8 rows and 2 blocks 145 us.
+template <int CH, int NV, bool WHOLE>
+constexpr int batch_rows() {
+  return NV * CH <= 4 ? (WHOLE ? 8 : 4) : (NV * CH <= 8 ? 4 : (NV * CH <= 16 ? 2 : 1));
+}
 template <int CH, int NV, bool WHOLE>
 constexpr int min_blocks() {
-  return CH * NV <= 4 ? (WHOLE ? 3 : 2) : (CH * NV <= 8 ? 2 : 1);
+  return CH * NV <= 4 ? 3 : (CH * NV <= 8 ? 2 : 1);
 }
 
 // ---- each node on its own: one warp per row, R rows in flight ----------------
@@ -334,18 +340,12 @@ __global__ void __launch_bounds__(kThreads, CH * NV <= 8 ? 4 : 1) norm_rows_kern
 
 // ---- graphs of a batch ------------------------------------------------------
 
-// rows of a warp in flight
-template <int CH, int NV>
-constexpr int batch_rows() {
-  return NV * CH <= 4 ? 8 : (NV * CH <= 8 ? 4 : (NV * CH <= 16 ? 2 : 1));
-}
-
 // The rows of a span, shared by a team: warp i of `size` takes rows i, i + size, ...
 // The team is the block, or a warp by itself.
 template <int CH, int NV, bool WHOLE>
 struct Team {
   static constexpr int E = WHOLE ? 1 : CH;
-  static constexpr int U = batch_rows<CH, NV>();
+  static constexpr int U = batch_rows<CH, NV, WHOLE>();
   Tile<CH, NV, WHOLE> t;
   float2* joint;  // [2][kWarps][groups in the tile]: (mean, M2) of the warps' rows
   int flip;       // which half of `joint` is next
