@@ -225,6 +225,10 @@ __device__ __forceinline__ void load_chunk(const float* p, float (&v)[CH]) {
     v[1] = t.y;
     v[2] = t.z;
     v[3] = t.w;
+  } else if constexpr (CH == 2) {
+    const float2 t = __ldg(reinterpret_cast<const float2*>(p));
+    v[0] = t.x;
+    v[1] = t.y;
   } else {
     v[0] = __ldg(p);
   }
@@ -234,6 +238,8 @@ template <int CH>
 __device__ __forceinline__ void store_chunk(float* p, const float (&v)[CH]) {
   if constexpr (CH == 4) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else if constexpr (CH == 2) {
+    *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
   } else {
     *p = v[0];
   }
@@ -568,6 +574,17 @@ __device__ __forceinline__ bool is_split(const NormArgs& a, int64_t s, int64_t e
   return e - s > kShort && s / a.window != (e - 1) / a.window;
 }
 
+// Asks the L2 for rows [r0, r1), whatever graphs they belong to.
+__device__ __forceinline__ void prefetch_rows(const NormArgs& a, int64_t r0, int64_t r1) {
+  const uintptr_t first = (reinterpret_cast<uintptr_t>(a.x + r0 * a.c) + 15) & ~uintptr_t(15);
+  const uintptr_t last = reinterpret_cast<uintptr_t>(a.x + r1 * a.c) & ~uintptr_t(15);
+  // (a few huge graphs stream anyway: no look-up to hide behind)
+  if (threadIdx.x == 0 && blockIdx.y == 0 && first < last && a.graphs * 8 >= a.windows) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(first), "r"(static_cast<uint32_t>(last - first))
+                 : "memory");
+  }
+}
+
 // Lists the graphs of rows [r0, r1) (in any order: no result depends on it); of the
 // long ones only the split ones where `split_only`.
 __device__ __forceinline__ void list_graphs(const NormArgs& a, int64_t r0, int64_t r1, bool split_only, Window& w) {
@@ -597,6 +614,7 @@ __global__ void __launch_bounds__(kThreads, min_blocks<CH, NV, WHOLE>()) norm_wi
   extern __shared__ float shared[];
   __shared__ Window list;
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.window, r1 = min(r0 + a.window, a.n);
+  prefetch_rows(a, r0, r1);
   list_graphs(a, r0, r1, false, list);
   Team<CH, NV, WHOLE> team;
   team.init(a, shared);
@@ -682,64 +700,83 @@ __device__ __forceinline__ double warp_sum(double v) {
 }
 
 // Joins the pieces of split graphs in 64 bits, always in the same order. Blocks with
-// blockIdx.y == 0 look through the graphs, 32 a warp at a time, and join those of few
-// pieces, a warp each; the others take the graphs of many pieces, a block per group.
+// blockIdx.y == 0 join graphs of few pieces, a warp each; the others take the graphs of
+// many pieces, a block per group.
 __global__ void __launch_bounds__(kThreads) norm_join_kernel(NormArgs a) {
   __shared__ double sh[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool few = blockIdx.y == 0;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * (few ? kThreads : 32);
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * (few ? kThreads : 32) + (few ? warp * 32 : 0);
-       base < a.graphs; base += stride) {
-    bool mine = false;
-    if (base + lane < a.graphs) {
-      const int64_t s = ptr_at(a, base + lane), e = ptr_at(a, base + lane + 1);
-      const bool many = e - s > static_cast<int64_t>(kFewPieces - 2) * a.window;
-      mine = is_split(a, s, e) && many != few;
-    }
-    for (unsigned todo = __ballot_sync(kFull, mine); todo != 0; todo &= todo - 1) {
-      const Pieces p(a, base + __ffs(todo) - 1);
-      if (few) {  // at most kFewPieces pieces
-        for (int grp = 0; grp < a.groups; ++grp) {
-          float2 v[2];
-          double size[2], sum = 0.0, m2 = 0.0;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int64_t k = p.first + lane + 32 * i;
-            v[i] = k <= p.last ? p.at(a, k, grp) : make_float2(0.0f, 0.0f);
-            size[i] = k <= p.last ? p.size(a, k) : 0.0;
-            sum += size[i] * v[i].x;
-          }
-          const double mean = warp_sum(sum) / p.total;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) m2 += v[i].y + size[i] * (v[i].x - mean) * (v[i].x - mean);
-          m2 = warp_sum(m2);
-          if (lane == 0) p.put(a, grp, mean, m2);
-        }
-      } else {
-        for (int grp = blockIdx.y - 1; grp < a.groups; grp += gridDim.y - 1) {
-          auto block_sum = [&](double v) {
-            v = warp_sum(v);
-            if (lane == 0) sh[warp] = v;
-            __syncthreads();
-            double t = 0.0;
-#pragma unroll
-            for (int i = 0; i < kWarps; ++i) t += sh[i];
-            __syncthreads();
-            return t;
-          };
+  if (blockIdx.y == 0) {
+    // lane l of warp w looks at graph w + l * warps, so that neighbours go to different warps
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarps;
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+    // the lanes are `parts` pieces times 32 / parts groups
+    int parts = 32;
+    while (parts > 1 && (32 / parts) < a.groups) parts /= 2;
+    const int width = 32 / parts, part = lane / width, col = lane & (width - 1);
+    for (int64_t base = 0; base < a.graphs; base += 32 * warps) {
+      const int64_t mine = base + w + lane * warps;
+      bool take = false;
+      if (mine < a.graphs) {
+        const int64_t s = ptr_at(a, mine), e = ptr_at(a, mine + 1);
+        take = is_split(a, s, e) && e - s <= static_cast<int64_t>(kFewPieces - 2) * a.window;
+      }
+      for (unsigned todo = __ballot_sync(kFull, take); todo != 0; todo &= todo - 1) {
+        const Pieces p(a, base + w + (__ffs(todo) - 1) * warps);
+        for (int g0 = 0; g0 < a.groups; g0 += width) {
+          const int grp = g0 + col;
+          const bool live = grp < a.groups;
           double sum = 0.0, m2 = 0.0;
 #pragma unroll 4
-          for (int64_t k = p.first + threadIdx.x; k <= p.last; k += kThreads) sum += p.size(a, k) * p.at(a, k, grp).x;
-          const double mean = block_sum(sum) / p.total;
-#pragma unroll 4
-          for (int64_t k = p.first + threadIdx.x; k <= p.last; k += kThreads) {
-            const float2 v = p.at(a, k, grp);
-            m2 += v.y + p.size(a, k) * (v.x - mean) * (v.x - mean);
+          for (int64_t k = p.first + part; k <= p.last; k += parts) {
+            if (live) sum += p.size(a, k) * p.at(a, k, grp).x;
           }
-          m2 = block_sum(m2);
-          if (threadIdx.x == 0) p.put(a, grp, mean, m2);
+          for (int o = width; o < 32; o <<= 1) sum += __shfl_xor_sync(kFull, sum, o);
+          const double mean = sum / p.total;
+#pragma unroll 4
+          for (int64_t k = p.first + part; k <= p.last; k += parts) {
+            if (live) {
+              const float2 v = p.at(a, k, grp);
+              m2 += v.y + p.size(a, k) * (v.x - mean) * (v.x - mean);
+            }
+          }
+          for (int o = width; o < 32; o <<= 1) m2 += __shfl_xor_sync(kFull, m2, o);
+          if (live && part == 0) p.put(a, grp, mean, m2);
         }
+      }
+    }
+    return;
+  }
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * 32; base < a.graphs;
+       base += static_cast<int64_t>(gridDim.x) * 32) {
+    bool take = false;
+    if (base + lane < a.graphs) {
+      const int64_t s = ptr_at(a, base + lane), e = ptr_at(a, base + lane + 1);
+      take = e - s > static_cast<int64_t>(kFewPieces - 2) * a.window;
+    }
+    for (unsigned todo = __ballot_sync(kFull, take); todo != 0; todo &= todo - 1) {  // the same in every warp
+      const Pieces p(a, base + __ffs(todo) - 1);
+      auto block_sum = [&](double v) {
+        v = warp_sum(v);
+        if (lane == 0) sh[warp] = v;
+        __syncthreads();
+        double t = 0.0;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) t += sh[i];
+        __syncthreads();
+        return t;
+      };
+      for (int grp = blockIdx.y - 1; grp < a.groups; grp += gridDim.y - 1) {
+        double sum = 0.0, m2 = 0.0;
+#pragma unroll 4
+        for (int64_t k = p.first + threadIdx.x; k <= p.last; k += kThreads) sum += p.size(a, k) * p.at(a, k, grp).x;
+        const double mean = block_sum(sum) / p.total;
+#pragma unroll 4
+        for (int64_t k = p.first + threadIdx.x; k <= p.last; k += kThreads) {
+          const float2 v = p.at(a, k, grp);
+          m2 += v.y + p.size(a, k) * (v.x - mean) * (v.x - mean);
+        }
+        m2 = block_sum(m2);
+        if (threadIdx.x == 0) p.put(a, grp, mean, m2);
       }
     }
   }
@@ -819,7 +856,7 @@ int run(const NormArgs& a, bool rows, unsigned tiles, cudaStream_t s) {
   norm_windows_kernel<CH, NV, WHOLE><<<grid, kThreads, smem, s>>>(a);
   GNN_LAUNCH_CHECK("norm_windows_kernel launch");
   if (a.n <= kShort) return GNN_OK;
-  const int64_t batches = (a.graphs + kThreads - 1) / kThreads;
+  const int64_t batches = (a.graphs + kWarps - 1) / kWarps;  // a warp per graph
   const bool many = a.n > static_cast<int64_t>(kFewPieces - 2) * a.window;  // some graph may have many pieces
   const dim3 jgrid(static_cast<unsigned>(std::min<int64_t>(batches, 4LL * sm_count())),
                    many ? 1u + static_cast<unsigned>(std::min(a.groups, 64)) : 1u);
@@ -837,10 +874,10 @@ int run_width(const NormArgs& a, bool rows, int64_t cols, unsigned tiles, cudaSt
   if (cols <= 64 * CH) return run<CH, 2, WHOLE>(a, rows, tiles, s);
   if (cols <= 128 * CH) return run<CH, 4, WHOLE>(a, rows, tiles, s);
   if (cols <= 256 * CH) return run<CH, 8, WHOLE>(a, rows, tiles, s);
-  if constexpr (CH == 1) {
-    if (cols <= 512) return run<CH, 16, WHOLE>(a, rows, tiles, s);
-    return run<CH, 32, WHOLE>(a, rows, tiles, s);
+  if constexpr (CH <= 2) {
+    if (cols <= 512 * CH) return run<CH, 16, WHOLE>(a, rows, tiles, s);
   }
+  if constexpr (CH == 1) return run<CH, 32, WHOLE>(a, rows, tiles, s);
   return fail(GNN_ERR_UNSUPPORTED, "group norm: column tile too wide");
 }
 
@@ -905,17 +942,18 @@ extern "C" int gnn_group_norm_forward(const float* x, const void* graph_ptr, int
     a.part = static_cast<float2*>(workspace);
     a.fin = a.part + a.windows * 2 * groups;
   }
-  // 16-byte pieces of rows: in several column tiles only where each starts on one
-  const bool vec = channels % 4 == 0 && (tiles == 1 || cg % 4 == 0) &&
-                   ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  // 16- or 8-byte pieces of rows: in several column tiles only where each starts on one
+  const uintptr_t base = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out);
+  const bool vec4 = channels % 4 == 0 && (tiles == 1 || cg % 4 == 0) && base % 16 == 0;
+  const bool vec2 = channels % 2 == 0 && (tiles == 1 || cg % 2 == 0) && base % 8 == 0;
   const int64_t cols = tile_groups * cg;
   const unsigned ty = static_cast<unsigned>(tiles);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int rc;
-  if (vec && cg % 4 == 0) {
-    rc = run_width<4, true>(a, rows, cols, ty, s);
-  } else if (vec) {
-    rc = run_width<4, false>(a, rows, cols, ty, s);
+  if (vec4) {
+    rc = cg % 4 == 0 ? run_width<4, true>(a, rows, cols, ty, s) : run_width<4, false>(a, rows, cols, ty, s);
+  } else if (vec2) {
+    rc = cg % 2 == 0 ? run_width<2, true>(a, rows, cols, ty, s) : run_width<2, false>(a, rows, cols, ty, s);
   } else {
     rc = run_width<1, true>(a, rows, cols, ty, s);
   }
