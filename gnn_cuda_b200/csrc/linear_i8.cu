@@ -43,7 +43,8 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int BM = 128;        // rows per tile (TMEM lanes)
 constexpr int KB = 128;        // K bytes per stage: one 128-byte swizzle row
 constexpr int kMaxStages = 8;
-constexpr size_t kSmemLimit = 227 * 1024;
+constexpr size_t kSmemLimit = 227 * 1024;  // per CTA
+constexpr size_t kSmemPerSm = 228 * 1024;
 constexpr int kBlockBytes = 32 * 32 * 4;  // one epilogue warp's staging: 32 rows x 128 bytes
 constexpr int64_t kMaxK = 131071;         // 128 * 128 * K stays below 2^31
 
@@ -122,20 +123,22 @@ struct Shape {
   static constexpr int kHalves = EW / 4;  // epilogue warps per TMEM lane quarter
   static constexpr int kCols = BN / kHalves >= 32 ? BN / kHalves : 32;  // columns per epilogue warp
   // staging buffers per warp: with two, a block is written while the last one leaves
-  static constexpr int kBuffers = OUT8 || EW == 16 || (BN == 256 && EW == 4) ? 1 : 2;
+  static constexpr int kBuffers = OUT8 || EW == 16 || BN == 64 || (BN == 256 && EW == 4) ? 1 : 2;
+  // CTAs per SM: narrow tiles move little each, so their latencies are overlapped instead
+  static constexpr int kCtas = BN <= 32 ? 3 : (BN <= 64 ? 2 : 1);
   static constexpr size_t fixed() {
     return 1024 /* alignment */ + EW * (kBuffers * kBlockBytes + kCols * 8) + (OUT8 ? kHalves * BM * 4 : 0) + 64;
   }
   static constexpr size_t bytes(int stages) { return fixed() + static_cast<size_t>(stages) * ((BM + BN) * KB + 16); }
   static constexpr int stages() {
     int s = kMaxStages;
-    while (bytes(s) > kSmemLimit) --s;
+    while (bytes(s) + 1024 > kSmemPerSm / kCtas || bytes(s) > kSmemLimit) --s;  // 1 KB a CTA is the system's
     return s;
   }
 };
 
 template <int BN, bool OUT8, int EW>
-__global__ void __launch_bounds__(64 + 32 * EW, 1)
+__global__ void __launch_bounds__(64 + 32 * EW, Shape<BN, OUT8, EW>::kCtas)
     linear_i8_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                      const __grid_constant__ CUtensorMap tmap_out, I8Params p) {
   using Sh = Shape<BN, OUT8, EW>;
@@ -615,7 +618,7 @@ int launch_bn(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int64_
       if (dev >= 0 && dev < 64) configured[dev] = true;
     }
   }
-  const int64_t ctas = std::min<int64_t>(p.m_tiles * p.n_tiles, sm_count());
+  const int64_t ctas = std::min<int64_t>(p.m_tiles * p.n_tiles, static_cast<int64_t>(Shape<BN, OUT8, EW>::kCtas) * sm_count());
   linear_i8_kernel<BN, OUT8, EW><<<static_cast<unsigned>(ctas), 64 + 32 * EW, smem, stream>>>(
       tx, tw, to, p);
   GNN_LAUNCH_CHECK("linear_i8_kernel launch");

@@ -4,7 +4,7 @@
 //
 // All three move each byte once. quantize_rows keeps a row's values in registers
 // between the maximum and the rounding (up to 1,024 columns, one warp a row, 4
-// rows of up to 128 columns in flight per warp); wider rows take a block and are
+// rows of up to 128 columns in flight per warp; 4,096 with a block a row); wider rows are
 // read a second time, from L1 / L2.
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -89,16 +89,51 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const float* __
   }
 }
 
-// One block per row, any width.
+// One block per row. Rows of up to kThreads * 16 columns stay in registers between the
+// maximum and the rounding; wider ones are read again. VEC as above.
+template <bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_wide_rows_kernel(const float* __restrict__ x, int64_t ldx,
                                                                       int64_t rows, int64_t cols,
                                                                       int8_t* __restrict__ q, int64_t ldq,
                                                                       float* __restrict__ scale) {
+  constexpr int kKeep = 4;  // groups of four columns a thread keeps
   __shared__ float part[kThreads / 32];
+  // column e of this thread's group g: four neighbours, or four a block apart
+  auto column = [](int64_t g, int e) -> int64_t {
+    return VEC ? (g * kThreads + threadIdx.x) * 4 + e : (g * 4 + e) * kThreads + threadIdx.x;
+  };
+  const int64_t groups = (cols + kThreads * 4 - 1) / (kThreads * 4);
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const float* src = x + r * ldx;
+    auto load = [&](int64_t g, float (&v)[4]) {
+      if constexpr (VEC) {
+        const int64_t c = column(g, 0);
+        const float4 t = c < cols ? __ldg(reinterpret_cast<const float4*>(src + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[0] = t.x;
+        v[1] = t.y;
+        v[2] = t.z;
+        v[3] = t.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = column(g, e) < cols ? __ldg(src + column(g, e)) : 0.0f;
+      }
+    };
+    float v[kKeep][4];
     float amax = 0.0f;
-    for (int64_t c = threadIdx.x; c < cols; c += kThreads) amax = max_abs_nan(amax, __ldg(src + c));
+#pragma unroll
+    for (int g = 0; g < kKeep; ++g) {
+      if (g < groups) {
+        load(g, v[g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) amax = max_abs_nan(amax, v[g][e]);
+      }
+    }
+    for (int64_t g = kKeep; g < groups; ++g) {
+      float t[4];
+      load(g, t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) amax = max_abs_nan(amax, t[e]);
+    }
     amax = warp_max_nan(amax);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
     __syncthreads();
@@ -106,7 +141,27 @@ __global__ void __launch_bounds__(kThreads) quantize_wide_rows_kernel(const floa
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) amax = max_abs_nan(amax, part[w]);
     const RowQuant rq = row_quant(amax);
-    for (int64_t c = threadIdx.x; c < cols; c += kThreads) q[r * ldq + c] = quant1(rq, __ldg(src + c));
+    int8_t* dst = q + r * ldq;
+    auto store = [&](int64_t g, const float (&t)[4]) {
+      const uint32_t p = quant4(rq, t[0], t[1], t[2], t[3]);
+      if constexpr (VEC) {
+        if (column(g, 0) < cols) *reinterpret_cast<uint32_t*>(dst + column(g, 0)) = p;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (column(g, e) < cols) dst[column(g, e)] = static_cast<int8_t>((p >> (8 * e)) & 0xffu);
+        }
+      }
+    };
+#pragma unroll
+    for (int g = 0; g < kKeep; ++g) {
+      if (g < groups) store(g, v[g]);
+    }
+    for (int64_t g = kKeep; g < groups; ++g) {
+      float t[4];
+      load(g, t);
+      store(g, t);
+    }
     if (threadIdx.x == 0) scale[r] = rq.s;
     __syncthreads();
   }
@@ -187,8 +242,10 @@ int quantize_rows(const float* x, int64_t ldx, int64_t rows, int64_t cols, int8_
     launch_rows<4>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
   } else if (cols <= 1024) {
     launch_rows<8>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+  } else if (vec) {
+    quantize_wide_rows_kernel<true><<<grid_for(rows), kThreads, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
   } else {
-    quantize_wide_rows_kernel<<<grid_for(rows), kThreads, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
+    quantize_wide_rows_kernel<false><<<grid_for(rows), kThreads, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
   }
   GNN_LAUNCH_CHECK("quantize_rows launch");
   return GNN_OK;

@@ -45,7 +45,7 @@ def _quantize(x):
 
 
 @pytest.mark.parametrize("rows,cols", [(1, 1), (5, 3), (33, 128), (1000, 127), (257, 200), (70, 501), (64, 1024),
-                                       (9, 1023), (7, 1025), (3, 5000), (40000, 64)])
+                                       (9, 1023), (7, 1025), (5, 1300), (6, 4096), (3, 5000), (4, 9001), (40000, 64)])
 def test_quantize_rows(rows, cols):
     x = _features(rows, cols, rows + cols)
     q, s = _quantize(x)
