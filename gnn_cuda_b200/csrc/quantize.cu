@@ -3,9 +3,8 @@
 // whose stride or base does not suit TMA.
 //
 // All three move each byte once. quantize_rows keeps a row's values in registers
-// between the maximum and the rounding (up to 1,024 columns, one warp a row, 4
-// rows of up to 128 columns in flight per warp; 4,096 with a block a row); wider rows are
-// read a second time, from L1 / L2.
+// between the maximum and the rounding (4 to 32 lanes a row up to 2,048 columns, a
+// block a row up to 4,096); wider rows are read a second time, from L1 / L2.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -26,27 +25,30 @@ __device__ __forceinline__ float warp_max_nan(float v) {
   return v;
 }
 
-// One warp per row, NV * 128 columns at most. VEC: cols % 4 == 0, x 16-byte and q
-// 4-byte aligned, row by row; lane l holds the float4 columns l + 32 j. Otherwise
-// lane l holds the columns l + 32 j, one by one.
-template <int NV, bool VEC>
+// LANES lanes per row, up to LANES * NV * 4 columns: lane l of them holds the columns
+// 4 (l + LANES j) .. + 4, so narrow rows share a warp. VEC: cols % 4 == 0, x 16-byte and
+// q 4-byte aligned, row by row. R warps' worth of rows are in flight.
+template <int LANES, int NV, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const float* __restrict__ x, int64_t ldx,
                                                                  int64_t rows, int cols, int8_t* __restrict__ q,
-                                                                 int64_t ldq, float* __restrict__ scale) {
-  constexpr int R = NV == 1 ? 4 : (NV == 2 ? 2 : 1);  // rows in flight per warp
-  const int lane = threadIdx.x & 31;
+                                                                 int64_t ldq, float* __restrict__ scale,
+                                                                 int word_store) {
+  constexpr int R = NV == 1 ? 4 : (NV == 2 ? 2 : 1);
+  constexpr int G = 32 / LANES;  // rows side by side in a warp
+  const int sub = threadIdx.x & (LANES - 1), side = (threadIdx.x & 31) / LANES;
   const int64_t warps = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
   const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  for (int64_t r0 = warp * R; r0 < rows; r0 += warps * R) {
+  for (int64_t r0 = warp * R * G; r0 < rows; r0 += warps * R * G) {
     float v[R][NV * 4];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const float* src = x + (r0 + i) * ldx;
-      const bool live = r0 + i < rows;
+      const int64_t row = r0 + i * G + side;
+      const float* src = x + row * ldx;
+      const bool live = row < rows;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
+        const int c = (sub + LANES * j) * 4;
         if constexpr (VEC) {
-          const int c = (lane + 32 * j) * 4;
           float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
           if (live && c < cols) t = __ldcs(reinterpret_cast<const float4*>(src + c));
           v[i][4 * j] = t.x;
@@ -55,36 +57,36 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const float* __
           v[i][4 * j + 3] = t.w;
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = lane + 32 * (4 * j + e);
-            v[i][4 * j + e] = (live && c < cols) ? __ldcs(src + c) : 0.0f;
-          }
+          for (int e = 0; e < 4; ++e) v[i][4 * j + e] = (live && c + e < cols) ? __ldg(src + c + e) : 0.0f;
         }
       }
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      if (r0 + i >= rows) break;
+      const int64_t row = r0 + i * G + side;
       float amax = 0.0f;
 #pragma unroll
       for (int j = 0; j < NV * 4; ++j) amax = max_abs_nan(amax, v[i][j]);
-      const RowQuant rq = row_quant(warp_max_nan(amax));
-      int8_t* dst = q + (r0 + i) * ldq;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const uint32_t p = quant4(rq, v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2], v[i][4 * j + 3]);
-        if constexpr (VEC) {
-          const int c = (lane + 32 * j) * 4;
-          if (c < cols) *reinterpret_cast<uint32_t*>(dst + c) = p;
-        } else {
+      for (int o = LANES / 2; o > 0; o >>= 1) amax = max_abs_nan(amax, __shfl_xor_sync(kFull, amax, o));
+      const RowQuant rq = row_quant(amax);
+      if (row < rows) {
+        int8_t* dst = q + row * ldq;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = lane + 32 * (4 * j + e);
-            if (c < cols) dst[c] = static_cast<int8_t>((p >> (8 * e)) & 0xffu);
+        for (int j = 0; j < NV; ++j) {
+          const uint32_t p = quant4(rq, v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2], v[i][4 * j + 3]);
+          const int c = (sub + LANES * j) * 4;
+          if (VEC ? c < cols : (word_store && c + 4 <= cols)) {
+            *reinterpret_cast<uint32_t*>(dst + c) = p;
+          } else if (!VEC) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (c + e < cols) dst[c + e] = static_cast<int8_t>((p >> (8 * e)) & 0xffu);
+            }
           }
         }
+        if (sub == 0) scale[row] = rq.s;
       }
-      if (lane == 0) scale[r0 + i] = rq.s;
     }
   }
 }
@@ -216,15 +218,18 @@ unsigned grid_for(int64_t units) {
   return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(units, 16LL * sm_count())));
 }
 
-template <int NV>
+template <int LANES, int NV>
 void launch_rows(bool vec, const float* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq,
                  float* scale, cudaStream_t stream) {
-  constexpr int per_block = (NV == 1 ? 4 : (NV == 2 ? 2 : 1)) * (kThreads / 32);
+  constexpr int per_block = (NV == 1 ? 4 : (NV == 2 ? 2 : 1)) * (32 / LANES) * (kThreads / 32);
   const unsigned grid = grid_for((rows + per_block - 1) / per_block);
+  const int word_store = ldq % 4 == 0 && reinterpret_cast<uintptr_t>(q) % 4 == 0;
   if (vec) {
-    quantize_rows_kernel<NV, true><<<grid, kThreads, 0, stream>>>(x, ldx, rows, static_cast<int>(cols), q, ldq, scale);
+    quantize_rows_kernel<LANES, NV, true>
+        <<<grid, kThreads, 0, stream>>>(x, ldx, rows, static_cast<int>(cols), q, ldq, scale, word_store);
   } else {
-    quantize_rows_kernel<NV, false><<<grid, kThreads, 0, stream>>>(x, ldx, rows, static_cast<int>(cols), q, ldq, scale);
+    quantize_rows_kernel<LANES, NV, false>
+        <<<grid, kThreads, 0, stream>>>(x, ldx, rows, static_cast<int>(cols), q, ldq, scale, word_store);
   }
 }
 
@@ -234,14 +239,22 @@ int quantize_rows(const float* x, int64_t ldx, int64_t rows, int64_t cols, int8_
                   cudaStream_t stream) {
   const bool vec = cols % 4 == 0 && ldx % 4 == 0 && ldq % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(q) % 4 == 0;
-  if (cols <= 128) {
-    launch_rows<1>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+  if (cols <= 16) {
+    launch_rows<4, 1>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+  } else if (cols <= 32) {
+    launch_rows<8, 1>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+  } else if (cols <= 64) {
+    launch_rows<16, 1>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+  } else if (cols <= 128) {
+    launch_rows<32, 1>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
   } else if (cols <= 256) {
-    launch_rows<2>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+    launch_rows<32, 2>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
   } else if (cols <= 512) {
-    launch_rows<4>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+    launch_rows<32, 4>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
   } else if (cols <= 1024) {
-    launch_rows<8>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+    launch_rows<32, 8>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
+  } else if (cols <= 2048) {
+    launch_rows<32, 16>(vec, x, ldx, rows, cols, q, ldq, scale, stream);
   } else if (vec) {
     quantize_wide_rows_kernel<true><<<grid_for(rows), kThreads, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
   } else {
