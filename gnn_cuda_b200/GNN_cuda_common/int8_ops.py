@@ -186,7 +186,7 @@ def linear_int8_forward_(x: torch.Tensor, x_scale: torch.Tensor | None, weight: 
         # Most calls on 8-bit rows need no scratch: the entry point says where one does, before it launches
         # anything. fp32 rows need it but for the fewest.
         rc = N.GNN_ERR_WORKSPACE
-        if x_scale is not None or m <= 8:
+        if x_scale is not None or m <= 16:
             rc = lib.gnn_linear_int8_forward(*args, None, 0, stream)
         if rc == N.GNN_ERR_WORKSPACE:
             wsb = lib.gnn_linear_int8_workspace_bytes(xp, x_type, ldx, wp, ldw, out_type, m, k, n)

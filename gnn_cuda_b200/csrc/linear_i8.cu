@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(64 + 32 * EW, Shape<BN, OUT8, EW>::kCtas)
 // is set up: one kernel quantises the rows (fp32 input; every block for itself, they
 // are small) into shared memory, zero-padded to 16 columns, and a warp takes an output
 // channel, 16 bytes of w a lane, with four-way 8-bit dot products.
-constexpr int kSmallRows = 8;
+constexpr int kSmallRows = 16;
 constexpr int kSmallBytes = 40 * 1024;  // shared memory for the rows
 constexpr int kSmallThreads = 256;
 
@@ -638,9 +638,14 @@ int launch(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int64_t k
   return launch_bn<256, OUT8, 16>(x, ldx, w, ldw, k, p, stream);
 }
 
-// Whether the few-rows kernel takes the call: fp32 output, aligned w, rows that fit.
+// Whether the few-rows kernel takes the call: fp32 output, aligned w, and rows so small
+// together that every block can quantise them for itself. Measured against the tile
+// kernel with its quantiser (fp32 rows, us on the device): K x N = 128 x 128, 16 rows 5.0 /
+// 7.5; 512 x 512, 16 rows 8.0 / 9.0, 17 rows 10.9 / 9.0; 1024 x 4096, 8 rows 11.4 / 11.0,
+// 16 rows 20.2 / 11.0.
 bool small_call(const int8_t* w, int64_t ldw, int out_type, int64_t m, int64_t k) {
-  return out_type == GNN_ROWS_FP32 && m <= kSmallRows && m * round_up(k, 16) <= kSmallBytes && aligned_rows(w, ldw);
+  return out_type == GNN_ROWS_FP32 && m <= kSmallRows && (m == 1 || m * k <= 8192) &&
+         m * round_up(k, 16) <= kSmallBytes && aligned_rows(w, ldw);
 }
 
 int launch_small(const SmallParams& p, cudaStream_t stream) {
@@ -653,8 +658,10 @@ int launch_small(const SmallParams& p, cudaStream_t stream) {
     linear_i8_small_kernel<2><<<grid, kSmallThreads, smem, stream>>>(p);
   } else if (p.m <= 4) {
     linear_i8_small_kernel<4><<<grid, kSmallThreads, smem, stream>>>(p);
-  } else {
+  } else if (p.m <= 8) {
     linear_i8_small_kernel<8><<<grid, kSmallThreads, smem, stream>>>(p);
+  } else {
+    linear_i8_small_kernel<16><<<grid, kSmallThreads, smem, stream>>>(p);
   }
   GNN_LAUNCH_CHECK("linear_i8_small_kernel launch");
   return GNN_OK;

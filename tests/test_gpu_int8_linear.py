@@ -91,7 +91,7 @@ def test_quantize_weight(k, n):
 
 
 SHAPES = [(1, 1, 1), (1, 512, 512), (3, 16, 7), (130, 128, 128), (1000, 501, 47), (257, 130, 33), (515, 64, 256),
-          (128 * 148 + 5, 128, 128), (300, 1000, 257), (64, 4096, 1000), (2, 1433, 7), (4, 130, 300), (8, 64, 64), (8, 5120, 40), (9, 40, 24), (129, 200, 640), (17, 2048, 96)]
+          (128 * 148 + 5, 128, 128), (300, 1000, 257), (64, 4096, 1000), (2, 1433, 7), (4, 130, 300), (8, 64, 64), (8, 5120, 40), (9, 40, 24), (16, 300, 40), (31, 1000, 65), (32, 1280, 300), (32, 1281, 20), (33, 64, 64), (129, 200, 640), (17, 2048, 96)]
 
 
 @pytest.mark.parametrize("m,k,n", SHAPES)
