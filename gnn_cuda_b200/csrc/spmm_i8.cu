@@ -11,6 +11,12 @@
 // share; what it holds of a row that began earlier, or ends later, goes to a
 // workspace slot, and a second small kernel adds those pieces in share order: no
 // float atomics, the same bits every time.
+//
+// Measured on one B200 (612,257 nodes, 16,077,042 entries, GCN, F = 128): 447 us and 25 us
+// for the pieces. Bound by instructions (0.66 a cycle and scheduler; unpacking and adding
+// 16 columns of an entry takes 36) and by the L2's gathers (2.06 GB of rows at 4.6 TB/s).
+// Against it: a whole warp per share with four columns a lane 684-790 us, lane groups on
+// one share joined at row ends 712 us, two rows in flight instead of four 521 us.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
