@@ -184,9 +184,9 @@ def linear_int8_forward_(x: torch.Tensor, x_scale: torch.Tensor | None, weight: 
 
     def call(stream):
         # Most calls on 8-bit rows need no scratch: the entry point says where one does, before it launches
-        # anything. fp32 rows need it but for the fewest.
+        # anything. fp32 rows need it but for the fewest (and then not for an 8-bit output).
         rc = N.GNN_ERR_WORKSPACE
-        if x_scale is not None or m <= 16:
+        if x_scale is not None or (m <= 16 and out_scale is None):
             rc = lib.gnn_linear_int8_forward(*args, None, 0, stream)
         if rc == N.GNN_ERR_WORKSPACE:
             wsb = lib.gnn_linear_int8_workspace_bytes(xp, x_type, ldx, wp, ldw, out_type, m, k, n)

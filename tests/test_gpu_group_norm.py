@@ -82,7 +82,7 @@ def _run(n, c, groups, ptr, act="none", seed=0, affine=True, index=torch.int32, 
         assert torch.equal(again, out)
 
 
-CHANNELS = [(1, 1), (5, 1), (12, 3), (12, 12), (21, 7), (64, 1), (64, 64), (96, 8), (100, 4), (128, 8), (128, 32),
+CHANNELS = [(1, 1), (5, 1), (27, 3), (32, 32), (32, 4), (100, 10), (128, 128), (64, 8), (60, 5), (48, 3), (12, 3), (12, 12), (21, 7), (64, 1), (64, 64), (96, 8), (100, 4), (128, 8), (128, 32),
             (130, 2), (192, 3), (256, 16), (300, 100), (512, 1), (999, 27), (1024, 1), (1023, 1), (1280, 10), (2050, 1025)]
 
 
@@ -95,6 +95,11 @@ def test_nodes(c, groups):
 def test_graphs(c, groups):
     n = 1000
     _run(n, c, groups, [0, 5, 5, 6, 70, 134, 135, 500, 980], seed=c + 1)
+
+
+@pytest.mark.parametrize("n,c,groups", [(1, 27, 3), (303, 27, 3), (20000, 9, 9), (70001, 14, 2), (5000, 128, 16)])
+def test_many_narrow_nodes(n, c, groups):
+    _run(n, c, groups, None, "relu", seed=n)
 
 
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
