@@ -460,16 +460,18 @@ int tc_status_read(int reset, int* status) {
 namespace gnnb200 {
 int spmm_status_read(int reset, int* status);  // spmm.cu
 int i8_status_read(int reset, int* status);    // linear_i8.cu
+int spmm_i8_status_read(int reset, int* status);  // spmm_i8.cu
 }
 
 extern "C" int gnn_device_status(int reset, int* status) {
   GNN_REQUIRE(status != nullptr, GNN_ERR_NULL_POINTER, "status must not be NULL");
-  int tc = 0, sp = 0, i8 = 0;
+  int tc = 0, sp = 0, i8 = 0, si8 = 0;
   int rc = gnnb200::tc_status_read(reset, &tc);
   if (rc == GNN_OK) rc = gnnb200::spmm_status_read(reset, &sp);
   if (rc == GNN_OK) rc = gnnb200::i8_status_read(reset, &i8);
+  if (rc == GNN_OK) rc = gnnb200::spmm_i8_status_read(reset, &si8);
   if (rc != GNN_OK) return rc;
-  *status = tc != 0 ? tc : (sp != 0 ? sp : i8);
+  *status = tc != 0 ? tc : (sp != 0 ? sp : (i8 != 0 ? i8 : si8));
   gnnb200::clear_error();
   return GNN_OK;
 }

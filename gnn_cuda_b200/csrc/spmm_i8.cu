@@ -12,6 +12,10 @@
 // workspace slot, and a second small kernel adds those pieces in share order: no
 // float atomics, the same bits every time.
 //
+// The entries are those that row_ptr spans, [row_ptr[0], row_ptr[n]), whatever the host
+// gives as their number: that one sizes the grid and the scratch and is the length of
+// col_ind and edge_weight, so entries past it count as absent and are recorded as a status.
+//
 // Measured on one B200 (612,257 nodes, 16,077,042 entries, GCN, F = 128): 447 us and 25 us
 // for the pieces. Bound by instructions (0.66 a cycle and scheduler; unpacking and adding
 // 16 columns of an entry takes 36) and by the L2's gathers (2.06 GB of rows at 4.6 TB/s).
@@ -31,6 +35,10 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTileCols = 512;  // columns of one pass (32 lanes x 16)
+
+// device status word: 0 ok, 39 row_ptr spans entries outside [0, num_edges)
+__device__ int g_spmm_i8_status = 0;
+constexpr int kSpanOutside = 39;
 
 enum Mode : int { kSum = GNN_WEIGHT_SUM, kMean = GNN_WEIGHT_MEAN, kGcn = GNN_WEIGHT_GCN, kWeighted = GNN_WEIGHT_EDGE };
 
@@ -118,30 +126,50 @@ __device__ __forceinline__ int64_t rp(const I8SpmmArgs& a, int64_t r) {
   return static_cast<int64_t>(__ldg(static_cast<const IdxT*>(a.row_ptr) + r));
 }
 
+// The rows of the CSR over the entries that exist: row r begins at(row_ptr[r]), counted from
+// the first entry, `base`; never below 0 nor past `span`, whatever row_ptr holds.
+template <class IdxT>
+struct Rows {
+  const IdxT* ptr;
+  IdxT base, end;
+  bool cut;  // row_ptr reaches outside the entries
+  __device__ __forceinline__ explicit Rows(const I8SpmmArgs& a) : ptr(static_cast<const IdxT*>(a.row_ptr)) {
+    const IdxT limit = static_cast<IdxT>(a.nnz), first = __ldg(ptr), last = __ldg(ptr + a.n);
+    base = min(max(first, IdxT(0)), limit);
+    end = min(max(last, base), limit);
+    cut = base != first || end != last;
+  }
+  __device__ __forceinline__ int64_t span() const { return static_cast<int64_t>(end - base); }
+  __device__ __forceinline__ int64_t at(IdxT v) const { return static_cast<int64_t>(min(max(v, base), end) - base); }
+  __device__ __forceinline__ int64_t begin(int64_t r) const { return at(__ldg(ptr + r)); }
+};
+
 // Number of row ends among the first `d` items of the merged sequence (row r's end
-// comes after its entries): the smallest r with row_ptr[r + 1] + r + 1 > d. The L
-// lanes of a group ask at L places a round; all groups of the warp take part.
+// comes after its entries): the smallest r with begin(r + 1) + r + 1 > d. The L
+// lanes of a group ask at L places a round; all groups of the warp take part. Past the
+// sequence's end it is n; the answer never exceeds d.
 template <int L, class IdxT>
-__device__ __forceinline__ int64_t row_at(const I8SpmmArgs& a, int64_t d) {
-  const int lane = threadIdx.x & 31, sub = lane & (L - 1);
-  int64_t lo = 0, hi = a.n;  // the answer is in [lo, hi]
-  while (__any_sync(kFull, lo < hi)) {
-    const int64_t step = (hi - lo + L - 1) / L;
-    const int64_t at = min(lo + sub * step + step - 1, hi - 1);
-    const bool past = lo < hi && rp<IdxT>(a, at + 1) + at + 1 > d;
-    const unsigned found = (__ballot_sync(kFull, past) >> (lane - sub)) & (L == 32 ? kFull : (1u << (L & 31)) - 1u);
-    if (lo < hi) {
-      if (found == 0) {
-        lo = hi;
-      } else {
-        const int64_t first = lo + (__ffs(found) - 1) * step;
-        hi = min(first + step - 1, hi - 1);
-        lo = step == 1 ? hi : min(first, hi);
-      }
+struct Search {
+  int64_t lo, hi;  // the answer is in [lo, hi]
+  __device__ __forceinline__ int64_t step() const { return (hi - lo + L - 1) / L; }
+  // the row at which this lane asks
+  __device__ __forceinline__ int64_t place() const {
+    return min(lo + ((threadIdx.x & (L - 1)) + 1) * step() - 1, hi - 1);
+  }
+  __device__ __forceinline__ void narrow(bool past) {
+    const unsigned all = __ballot_sync(kFull, lo < hi && past);
+    const unsigned found = (all >> (threadIdx.x & 31 & ~(L - 1))) & (L == 32 ? kFull : (1u << (L & 31)) - 1u);
+    if (lo >= hi) return;
+    const int64_t s = step();
+    if (found == 0) {
+      lo = hi;
+    } else {
+      const int64_t first = lo + (__ffs(found) - 1) * s;
+      hi = min(first + s - 1, hi - 1);
+      lo = s == 1 ? hi : min(first, hi);
     }
   }
-  return lo;
-}
+};
 
 template <class IdxT>
 __device__ __forceinline__ float row_factor(const I8SpmmArgs& a, int64_t r) {
@@ -168,7 +196,7 @@ template <int L, int KIND, class IdxT>
 __global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
   constexpr int U = 4;
   const int sub = threadIdx.x & (L - 1);
-  const int64_t w = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / L;  // share
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * (kThreads / L) + threadIdx.x / L;  // share
   // this lane's 16 columns; a lane past the last one reads the first ones and stores nothing
   const int c0 = blockIdx.y * kTileCols + sub * 16;  // f > 512: column tiles
   const bool have = c0 < a.f;
@@ -176,27 +204,40 @@ __global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
   const int8_t* const xl = a.x + cl;
   const uint32_t ldx = static_cast<uint32_t>(a.ldx);
   const int last_row = static_cast<int>(a.n - 1);
-  // a group past the last share takes an empty one
-  const int64_t total = a.n + a.nnz;
-  const int64_t d0 = min(w * a.share, total), d1 = min(d0 + a.share, total);
-  int row = static_cast<int>(row_at<L, IdxT>(a, d0));
-  const int row_end = static_cast<int>(row_at<L, IdxT>(a, d1));  // rows [row, row_end) end in this share
-  const int64_t e0 = d0 - row;
-  const int len = static_cast<int>(d1 - row_end - e0);  // entries; positions are relative to e0
-  bool head = row < a.n && rp<IdxT>(a, row) < e0;       // the first row began in an earlier share
-  const bool open = e0 + len > max(e0, rp<IdxT>(a, row_end));  // the last entries' row ends in a later share
+  const Rows<IdxT> rows(a);
+  if (rows.cut && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+    atomicCAS(&g_spmm_i8_status, 0, kSpanOutside);
+  }
+  // a group past the last share, or past the entries that row_ptr spans, takes an empty one
+  const int64_t d0 = w * a.share, d1 = d0 + a.share;
+  Search<L, IdxT> begins{0, a.n}, ends{0, a.n};  // both at once: their loads are on their way together
+  while (__any_sync(kFull, begins.lo < begins.hi || ends.lo < ends.hi)) {
+    const int64_t r0 = begins.place(), r1 = ends.place();
+    const int64_t v0 = rows.begin(r0 + 1), v1 = rows.begin(r1 + 1);
+    begins.narrow(v0 + r0 + 1 > d0);
+    ends.narrow(v1 + r1 + 1 > d1);
+  }
+  int row = static_cast<int>(begins.lo);
+  const int row_end = max(row, static_cast<int>(ends.lo));  // rows [row, row_end) end in this share
+  const int64_t e0 = min(d0 - row, rows.span());
+  // entries; positions are relative to e0
+  const int len = static_cast<int>(max(min(d1 - row_end, rows.span()) - e0, int64_t(0)));
+  bool head = row < a.n && rows.begin(row) < e0;            // the first row began in an earlier share
+  const bool open = e0 + len > max(e0, rows.begin(row_end));  // the last entries' row ends in a later share
   if (sub == 0 && blockIdx.y == 0 && w < a.shares) {
     // the row that this share begins but does not end: its piece is the tail slot
     a.part_row[w] = open && !(head && row == row_end) ? row_end : -1;
   }
-  const int32_t* const cp = a.col + e0 + sub;
+  const IdxT entry = rows.base + static_cast<IdxT>(e0);  // the share's first entry
+  const int32_t* const cp = a.col + entry + sub;
   auto load_col = [&](int p) -> int { return p + sub < len ? ld_stream_i32(cp + p) : 0; };
   // past the share: weight 0 on row 0
   auto load_weight = [&](int p, int c) -> float {
-    return p + sub < len ? entry_weight(a, c, e0 + p + sub) : 0.0f;
+    return p + sub < len ? entry_weight(a, c, static_cast<int64_t>(entry) + p + sub) : 0.0f;
   };
+  // (past len, so that the row ends behind the loop, where the entries are cut off)
   auto load_stop = [&](int r) -> int {
-    return r < row_end ? static_cast<int>(rp<IdxT>(a, r + 1) - e0) : 0x7fffffff;
+    return r < row_end ? static_cast<int>(__ldg(static_cast<const IdxT*>(a.row_ptr) + r + 1) - entry) : 0x7fffffff;
   };
   auto load_factor = [&](int r) -> float { return r < row_end ? row_factor<IdxT>(a, r) : 0.0f; };
   float* const partl = a.part + 2 * w * a.f + c0;
@@ -280,10 +321,11 @@ __global__ void __launch_bounds__(kThreads) spmm_i8_join_kernel(I8SpmmArgs a) {
   const int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   if (w >= a.shares) return;
   const int64_t row = a.part_row[w];
+  const Rows<IdxT> rows(a);
   const int c = blockIdx.y * 32 + (threadIdx.x & 31);
-  if (row < 0 || c >= a.f) return;
-  // the row's end is item row_ptr[row + 1] + row of the merged sequence
-  const int64_t last = (rp<IdxT>(a, row + 1) + row) / a.share;
+  if (row < 0 || row >= a.n || c >= a.f) return;
+  const int64_t end = rows.begin(row + 1);
+  const int64_t last = (end + row) / a.share;  // the row's end is item end + row of the merged sequence
   const float* p = a.part + 2 * w * a.f + c;
   float s = p[a.f];
   int64_t k = w + 1;
@@ -362,6 +404,16 @@ int run(const I8SpmmArgs& a, cudaStream_t s) {
 }
 
 }  // namespace
+
+int spmm_i8_status_read(int reset, int* status) {
+  GNN_CUDA_TRY(cudaMemcpyFromSymbol(status, g_spmm_i8_status, sizeof(int)), "read 8-bit aggregation status word");
+  if (reset) {
+    const int zero = 0;
+    GNN_CUDA_TRY(cudaMemcpyToSymbol(g_spmm_i8_status, &zero, sizeof(int)), "reset 8-bit aggregation status word");
+  }
+  return GNN_OK;
+}
+
 }  // namespace gnnb200
 
 using namespace gnnb200;

@@ -89,8 +89,9 @@ int gnn_gemm_uses_tensor_cores(int64_t m, int64_t k, int64_t n);
  * segment chain of long rows in the aggregation kernels) give up after ~2 s
  * instead of hanging; they then record a non-zero code here (1-6 tensor-core
  * pipeline, 16 aggregation segment chain, 17 aggregation long-row list
- * overflow, 33-38 8-bit transform pipeline) and the kernel moves on. Synchronises with the current device,
- * stores the word in *status and clears it when reset != 0. */
+ * overflow, 33-38 8-bit transform pipeline) and the kernel moves on. 39: row_ptr of an
+ * aggregation over 8-bit rows spans entries outside [0, num_edges). Synchronises with the
+ * current device, stores the word in *status and clears it when reset != 0. */
 int gnn_device_status(int reset, int* status);
 
 /* ---- CSR aggregation (SpMM) ------------------------------------------------
@@ -330,7 +331,10 @@ typedef enum gnn_weighting {
 /* The aggregations of gnn_spmm_*_forward over 8-bit rows: out[r, :] (fp32, [num_nodes,
  * feat_dim], contiguous) = f_r * sum_e w_e * x_scale[c] * x[c, :] in fp32. x is
  * [num_nodes, feat_dim] with row stride ldx; deg_inv_sqrt / edge_weight as the
- * weighting needs, else NULL. Deterministic, no atomics; the order of a row's sum
+ * weighting needs, else NULL. The entries are those of [row_ptr[0], row_ptr[num_nodes]);
+ * num_edges is the length of col_ind (and edge_weight), which may hold others before and
+ * behind them. Entries past num_edges count as absent (not in a mean's degree) and set
+ * the status word (39, gnn_device_status). Deterministic, no floating-point atomics; the order of a row's sum
  * differs from the fp32 entry points. Where x's base and ldx are multiples of 16 its
  * rows are read in whole 16-byte pieces, so every row but the last must be backed by
  * its full stride. Calls in flight at once need workspaces of their own

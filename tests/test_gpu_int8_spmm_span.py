@@ -1,0 +1,99 @@
+"""The aggregation over 8-bit rows takes its entries from row_ptr (run with -m gpu).
+
+col_ind and edge_weight may be longer than what row_ptr spans, before its first entry and
+behind its last; out is the middle of a filled buffer, whose rest must stay as it is.
+
+Bound as in test_gpu_int8_spmm.py: (d + 4) * 2^-24 * sum_e |w_e s_c q_c| for a row of d
+entries, 1.01 for the higher orders.
+"""
+import ctypes
+
+import numpy as np
+import pytest
+import scipy.sparse as sp
+import torch
+
+from gnn_cuda_b200 import _native as N
+from gnn_cuda_b200.GNN_cuda_common import int8_ops as I
+from tests import int8_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+FILL = 12345.0
+OUTSIDE = 39  # status: row_ptr spans entries outside col_ind
+
+
+def _status():
+    status = ctypes.c_int(-1)
+    N.check(N.lib().gnn_device_status(1, ctypes.byref(status)))
+    return status.value
+
+
+def _run(degrees, f, agg, index, front=0, slack=0, seed=1):
+    """The CSR of `degrees` with `front` foreign entries before it and `slack` behind it; entries
+    that a negative slack cuts off do not count."""
+    r = np.random.default_rng(seed)
+    n = len(degrees)
+    rp = front + np.concatenate([[0], np.cumsum(degrees)])
+    size = rp[-1] + slack
+    col = r.integers(0, n, size).astype(np.int32)
+    ew = r.standard_normal(size).astype(np.float32)
+    q, s = O.quantize(r.standard_normal((n, f)).astype(np.float32))
+    dis = r.random(n).astype(np.float32) + np.float32(0.1)
+    held = np.minimum(rp, size)  # rows over the entries that exist
+    deg = np.diff(held)
+    row = np.repeat(np.arange(n), deg)
+    c = col[held[0]:held[-1]]
+    w = s[c].astype(np.float64)
+    if agg == "gcn":
+        w = w * dis[row] * dis[c]
+    elif agg == "weighted":
+        w = w * ew[held[0]:held[-1]]
+    elif agg == "mean":
+        w = w / deg[row]
+    a = sp.csr_matrix((w, c, held - held[0]), shape=(n, n), copy=True)
+    want, size_ = a @ q.astype(np.float64), abs(a) @ np.abs(q.astype(np.float64))
+    x = I.empty_rows(n, f, DEV)
+    x.copy_(torch.from_numpy(q))
+    around = torch.full((n + 8, f), FILL, device=DEV)
+    out = around[4:4 + n]
+    I.spmm_int8_forward_(torch.from_numpy(rp.astype(index)).to(DEV), torch.from_numpy(col).to(DEV), x,
+                         torch.from_numpy(s).to(DEV), out, aggregation=agg,
+                         deg_inv_sqrt=torch.from_numpy(dis).to(DEV) if agg == "gcn" else None,
+                         edge_weight=torch.from_numpy(ew).to(DEV) if agg == "weighted" else None)
+    err = np.abs(out.cpu().numpy().astype(np.float64) - want)
+    assert np.all(err <= 1.01 * (deg[:, None] + 4) * 2.0 ** -24 * size_)
+    assert bool((around[:4] == FILL).all()) and bool((around[4 + n:] == FILL).all())
+
+
+def _degrees(n, seed=3):
+    r = np.random.default_rng(seed)
+    d = r.integers(0, 9, n)
+    d[n // 3] = 900  # a row over several shares
+    return d
+
+
+@pytest.mark.parametrize("index", [np.int32, np.int64])
+@pytest.mark.parametrize("agg", ["sum", "mean", "gcn", "weighted"])
+@pytest.mark.parametrize("front,slack", [(0, 0), (0, 1), (0, 1000), (5, 0), (5, 1), (700, 1000)])
+def test_entries_outside_the_rows(agg, index, front, slack):
+    _run(_degrees(501), 40, agg, index, front, slack)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("n,deg", [(1, 0), (1, 1), (40, 3), (64, 1)])
+@pytest.mark.parametrize("f", [1, 128, 300])
+def test_small_graphs_with_slack(n, deg, f):
+    _run(np.full(n, deg), f, "mean", np.int32, 2, 1)
+    _run(np.full(n, deg), f, "gcn", np.int64, 0, 33)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("index", [np.int32, np.int64])
+@pytest.mark.parametrize("missing", [1, 33, 1500])
+def test_fewer_entries_than_row_ptr_spans(index, missing):
+    """The rows hold what there is, and the status word says so."""
+    assert _status() == 0
+    _run(_degrees(501), 40, "weighted", index, 0, -missing)
+    assert _status() == OUTSIDE
+    assert _status() == 0
