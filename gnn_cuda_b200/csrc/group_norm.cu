@@ -23,6 +23,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
@@ -873,12 +874,22 @@ __global__ void __launch_bounds__(kThreads, min_blocks<CH, NV, WHOLE>()) norm_ap
   }
 }
 
-// Opts a kernel in to more than 48 KB of dynamic shared memory where it needs it.
-template <class Kernel>
-int allow_shared(Kernel kernel, size_t bytes) {
+// Opts a kernel in to more than 48 KB of dynamic shared memory where a call needs it: once
+// per device, to the most that any call can need, so that no thread takes away what
+// another is about to launch with.
+template <auto Kernel>
+int allow_shared(size_t bytes, size_t most) {
   if (bytes <= 48 * 1024) return GNN_OK;
-  GNN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)),
-               "group norm: shared memory opt-in");
+  static bool configured[64] = {};
+  static std::mutex mu;
+  int dev = 0;
+  GNN_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
+  std::lock_guard<std::mutex> lock(mu);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    GNN_CUDA_TRY(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)),
+                 "group norm: shared memory opt-in");
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
   return GNN_OK;
 }
 
@@ -905,14 +916,16 @@ int run(const NormArgs& a, bool rows, unsigned tiles, cudaStream_t s) {
     constexpr int R = NV * CH <= 4 ? 4 : (NV * CH <= 8 ? 2 : 1);
     const int64_t want = (a.n + kWarps * R - 1) / (kWarps * R);
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(want, 16LL * sm_count())), tiles);
-    if (int rc = allow_shared(norm_rows_kernel<CH, NV, WHOLE>, warps)) return rc;
+    if (int rc = allow_shared<norm_rows_kernel<CH, NV, WHOLE>>(warps, warps)) return rc;
     norm_rows_kernel<CH, NV, WHOLE><<<grid, kThreads, warps, s>>>(a);
     GNN_LAUNCH_CHECK("norm_rows_kernel launch");
     return GNN_OK;
   }
   const size_t smem = warps + sizeof(float2) * 2 * kWarps * a.tile_groups;
+  constexpr size_t most = sizeof(float) * kWarps * scratch_floats<CH, NV, WHOLE>() + sizeof(float2) * 2 * kWarps * kTile;
+  static_assert(most + sizeof(Window) + 1024 <= 227 * 1024, "the largest call has to fit");
   const dim3 grid(static_cast<unsigned>(a.windows), tiles);
-  if (int rc = allow_shared(norm_windows_kernel<CH, NV, WHOLE>, smem)) return rc;
+  if (int rc = allow_shared<norm_windows_kernel<CH, NV, WHOLE>>(smem, most)) return rc;
   norm_windows_kernel<CH, NV, WHOLE><<<grid, kThreads, smem, s>>>(a);
   GNN_LAUNCH_CHECK("norm_windows_kernel launch");
   if (a.n <= kShort) return GNN_OK;
@@ -922,7 +935,7 @@ int run(const NormArgs& a, bool rows, unsigned tiles, cudaStream_t s) {
                    many ? 1u + static_cast<unsigned>(std::min(a.groups, 64)) : 1u);
   norm_join_kernel<<<jgrid, kThreads, 0, s>>>(a);
   GNN_LAUNCH_CHECK("norm_join_kernel launch");
-  if (int rc = allow_shared(norm_apply_kernel<CH, NV, WHOLE>, smem)) return rc;
+  if (int rc = allow_shared<norm_apply_kernel<CH, NV, WHOLE>>(smem, most)) return rc;
   norm_apply_kernel<CH, NV, WHOLE><<<grid, kThreads, smem, s>>>(a);
   GNN_LAUNCH_CHECK("norm_apply_kernel launch");
   return GNN_OK;
