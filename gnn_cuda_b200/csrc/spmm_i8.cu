@@ -236,10 +236,13 @@ __global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
     return p + sub < len ? entry_weight(a, c, static_cast<int64_t>(entry) + p + sub) : 0.0f;
   };
   // (past len, so that the row ends behind the loop, where the entries are cut off)
-  auto load_stop = [&](int r) -> int {
-    return r < row_end ? static_cast<int>(__ldg(static_cast<const IdxT*>(a.row_ptr) + r + 1) - entry) : 0x7fffffff;
+  // (r unsigned: one past the last of 2^31 - 1 rows is no negative place)
+  auto load_stop = [&](uint32_t r) -> int {
+    return r < static_cast<uint32_t>(row_end) ? static_cast<int>(__ldg(static_cast<const IdxT*>(a.row_ptr) + r + 1) - entry) : 0x7fffffff;
   };
-  auto load_factor = [&](int r) -> float { return r < row_end ? row_factor<IdxT>(a, r) : 0.0f; };
+  auto load_factor = [&](uint32_t r) -> float {
+    return r < static_cast<uint32_t>(row_end) ? row_factor<IdxT>(a, r) : 0.0f;
+  };
   float* const partl = a.part + 2 * w * a.f + c0;
   const bool vec = (a.f & 7) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
   uint64_t acc[8];
@@ -268,8 +271,8 @@ __global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
     }
   };
   // where the current row and the next one end, and their factors
-  int stop = load_stop(row), stop_nxt = load_stop(row + 1);
-  float factor = load_factor(row), factor_nxt = load_factor(row + 1);
+  int stop = load_stop(row), stop_nxt = load_stop(row + 1u);
+  float factor = load_factor(row), factor_nxt = load_factor(row + 1u);
   auto finish_row = [&]() {
     // the row's sums, or the piece of a row that began earlier
     store(head ? partl : a.out + static_cast<int64_t>(row) * a.f + c0, head ? 1.0f : factor);
@@ -277,8 +280,8 @@ __global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
     ++row;
     stop = stop_nxt;
     factor = factor_nxt;
-    stop_nxt = load_stop(row + 1);
-    factor_nxt = load_factor(row + 1);
+    stop_nxt = load_stop(row + 1u);
+    factor_nxt = load_factor(row + 1u);
   };
 
   int c_cur = load_col(0);

@@ -97,3 +97,26 @@ def test_fewer_entries_than_row_ptr_spans(index, missing):
     _run(_degrees(501), 40, "weighted", index, 0, -missing)
     assert _status() == OUTSIDE
     assert _status() == 0
+
+
+def test_as_many_nodes_as_are_accepted():
+    """2^31 - 1 nodes: the rows behind the last one are not looked up at negative places."""
+    n, deg = (1 << 31) - 1, 5
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    rp = torch.zeros(n + 1, dtype=torch.int32, device=DEV)
+    rp[-1] = deg
+    col = torch.tensor([n - 1, 0, n - 2, n - 1, 7], dtype=torch.int32, device=DEV)
+    x = torch.zeros(n, 1, dtype=torch.int8, device=DEV)
+    x[-2:, 0] = torch.tensor([3, -100], dtype=torch.int8, device=DEV)
+    x[0], x[7] = 11, 1
+    s = torch.full((n,), 0.5, device=DEV)
+    out = torch.ones(n, 1, device=DEV)
+    I.spmm_int8_forward_(rp, col, x, s, out)
+    assert float(out[-1]) == 0.5 * (-100 + 11 + 3 - 100 + 1)
+    assert int(torch.count_nonzero(out[:-1])) == 0
+    assert _status() == 0
+    with pytest.raises(RuntimeError, match="2\\^31 - 1"):
+        N.check(N.lib().gnn_spmm_int8_forward(rp.data_ptr(), N.GNN_INDEX_INT32, col.data_ptr(), N.GNN_WEIGHT_SUM, None,
+                                              None, x.data_ptr(), 1, s.data_ptr(), out.data_ptr(), n + 1, deg, 1, None,
+                                              0, None))
