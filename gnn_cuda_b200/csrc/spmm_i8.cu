@@ -270,12 +270,13 @@ __global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
       }
     }
   };
-  // where the current row and the next one end, and their factors
+  // where the current row and the next one end, and their factors; a row without entries is 0,
+  // also where its factor is no number (the GCN factor of degree 0)
   int stop = load_stop(row), stop_nxt = load_stop(row + 1u);
-  float factor = load_factor(row), factor_nxt = load_factor(row + 1u);
-  auto finish_row = [&]() {
+  float factor = min(stop, len) > 0 || head ? load_factor(row) : 0.0f, factor_nxt = load_factor(row + 1u);
+  auto finish_row = [&](bool any) {
     // the row's sums, or the piece of a row that began earlier
-    store(head ? partl : a.out + static_cast<int64_t>(row) * a.f + c0, head ? 1.0f : factor);
+    store(head ? partl : a.out + static_cast<int64_t>(row) * a.f + c0, head ? 1.0f : (any ? factor : 0.0f));
     head = false;
     ++row;
     stop = stop_nxt;
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const float wt = __shfl_sync(kFull, w_cur, j + u, L);
-        while (stop == base + j + u && row < row_end) finish_row();
+        for (bool any = true; stop == base + j + u && row < row_end; any = false) finish_row(any);
         const uint64_t ww = pair(wt, wt);
         fma_word(ww, v[u].x, acc[0], acc[1]);
         fma_word(ww, v[u].y, acc[2], acc[3]);
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
     w_cur = w_nxt;
     c_nxt = c_far;
   }
-  while (row < row_end) finish_row();               // rows that end with the share's last entry
+  for (bool any = true; row < row_end; any = false) finish_row(any);               // rows that end with the share's last entry
   if (open) store(head ? partl : partl + a.f, 1.0f);  // entries of a row that ends in a later share
 }
 

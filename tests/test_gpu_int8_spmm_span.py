@@ -120,3 +120,27 @@ def test_as_many_nodes_as_are_accepted():
         N.check(N.lib().gnn_spmm_int8_forward(rp.data_ptr(), N.GNN_INDEX_INT32, col.data_ptr(), N.GNN_WEIGHT_SUM, None,
                                               None, x.data_ptr(), 1, s.data_ptr(), out.data_ptr(), n + 1, deg, 1, None,
                                               0, None))
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("kind", ["alternate", "runs", "ends", "none"])
+def test_rows_without_entries_whose_factor_is_infinite(kind, index):
+    """deg_inv_sqrt = degree^-0.5 is infinite for isolated nodes, whose rows are 0, as in the fp32 aggregation."""
+    from gnn_cuda_b200.GNN_cuda_common import gcn_ops
+    n, f = 2003, 48
+    r = np.random.default_rng(4)
+    deg = {"alternate": np.arange(n) % 2 * 3, "runs": (np.arange(n) // 70 % 2) * r.integers(1, 9, n),
+           "ends": np.where((np.arange(n) < 90) | (np.arange(n) > n - 40), 0, 2), "none": np.zeros(n, np.int64)}[kind]
+    rp = torch.from_numpy(np.concatenate([[0], np.cumsum(deg)])).to(DEV, index)
+    full = np.flatnonzero(deg) if deg.any() else np.zeros(1, np.int64)
+    col = torch.from_numpy(r.choice(full, int(deg.sum())).astype(np.int32)).to(DEV)
+    dis = torch.from_numpy(deg).to(DEV).float().pow(-0.5)
+    x = torch.randint(-127, 128, (n, f), device=DEV).to(torch.int8)
+    s = torch.rand(n, device=DEV)
+    out, ref = torch.empty(n, f, device=DEV), torch.empty(n, f, device=DEV)
+    I.spmm_int8_forward_(rp, col, x, s, out, aggregation="gcn", deg_inv_sqrt=dis)
+    gcn_ops.spmm_gcn_forward_(rp, col, dis, x.float() * s[:, None], ref)
+    empty = torch.from_numpy(deg == 0).to(DEV)
+    assert int(torch.count_nonzero(out[empty])) == 0 and int(torch.count_nonzero(ref[empty])) == 0
+    # both sides: 8 additions, the product by the scale and three of weights, each 2^-24 of at most 127 per entry
+    assert float((out - ref).abs().max()) <= 2 * 12 * 2.0 ** -24 * 127 * 9
