@@ -1,0 +1,55 @@
+"""How exact the group norm is where a coarse step would show (run with -m gpu).
+
+u = 2^-24 throughout; references in 64 bits.
+"""
+import pytest
+import torch
+
+from gnn_cuda_b200.GNN_cuda_common import norm_ops as M
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+U = 2.0 ** -24
+EPS = 1e-5
+
+
+def _activated(y, act):
+    """act(y): weight 0 leaves the bias as the activation's argument."""
+    c = y.numel()
+    x = torch.randn(3, c, device=DEV)
+    out = torch.empty_like(x)
+    M.group_norm_forward_(x, c // 64, torch.zeros(c, device=DEV), y, out, activation=act)
+    assert torch.equal(out[0], out[1]) and torch.equal(out[0], out[2])
+    return out[0].double()
+
+
+def test_gelu_relative_error():
+    """y Phi(y) = max(y, 0) - z Phi(-z), z = |y|. The fit of Phi(-z) exp(z^2 / 2) is off by 1.4e-7 of itself; its two
+    polynomials, their quotient, the exponential (two units) and the products are below 20 roundings; the exponent
+    z^2 / 2 carries three. For y > 0 two more roundings of the result come on top, and Phi(-z) is below it."""
+    y = torch.linspace(-8, 8, 4096, device=DEV)
+    d = y.double()
+    want = d * 0.5 * torch.special.erfc(-d / 2 ** 0.5)
+    rel = 1.4e-7 + (20 + 1.5 * d * d) * U
+    tail = d.abs() * 0.5 * torch.special.erfc(d.abs() / 2 ** 0.5)
+    bound = rel * tail + torch.where(d > 0, 2 * U * want, torch.zeros_like(d))
+    assert bool(((_activated(y, "gelu") - want).abs() <= bound).all())
+
+
+def test_gelu_special_values():
+    inf = float("inf")
+    y = torch.tensor([0.0, -0.0, 30.0, -30.0, inf, float("nan"), 1e30, -1e30] * 64, device=DEV)
+    got = torch.empty(2, y.numel(), device=DEV)
+    M.group_norm_forward_(torch.randn(2, y.numel(), device=DEV), 8, torch.zeros(y.numel(), device=DEV), y, got,
+                          activation="gelu")
+    row = got[0, :8].tolist()
+    assert row[0] == 0 and row[1] == 0 and row[2] == 30 and row[3] == 0 and row[4] == inf
+    assert row[5] != row[5] and row[6] == torch.tensor(1e30).item() and row[7] == 0
+
+
+def test_silu_relative_error():
+    """The exponential's argument, |y| log2 e, is rounded twice; two units each for it and the quotient, two sums."""
+    y = torch.linspace(-80, 40, 4096, device=DEV)
+    d = y.double()
+    want = d / (1 + torch.exp(-d))
+    assert bool(((_activated(y, "silu") - want).abs() <= (2 * d.abs() + 12) * U * want.abs()).all())
