@@ -53,3 +53,23 @@ def test_silu_relative_error():
     d = y.double()
     want = d / (1 + torch.exp(-d))
     assert bool(((_activated(y, "silu") - want).abs() <= (2 * d.abs() + 12) * U * want.abs()).all())
+
+
+# narrow nodes (few channels), then a warp per row: pieces of 16, 8 and 4 bytes, one and several column tiles
+@pytest.mark.parametrize("c,groups", [(16, 8), (27, 9), (12, 3), (63, 21), (192, 96), (300, 100), (256, 64), (512, 128),
+                                      (1024, 512), (262, 131), (1050, 350), (201, 67), (2050, 1025), (4100, 1025)])
+def test_groups_of_few_near_values(c, groups):
+    """Values 3 + 0.001 t: differences from the group's first value are exact (they are within a factor of two), so
+    every step is rounded in proportion to their largest, D: cg sums, a product, two subtractions."""
+    n = 3000
+    x = 3 + 1e-3 * torch.randn(n, c, device=DEV)
+    out = torch.empty_like(x)
+    M.group_norm_forward_(x, groups, None, None, out)
+    v = x.double().view(n, groups, -1)
+    cg = c // groups
+    d = v - v.mean(2, keepdim=True)
+    sd = (d.square().mean(2, keepdim=True) + EPS).sqrt()
+    z = d / sd
+    big = (v - v[:, :, :1]).abs().amax(2, keepdim=True)
+    bound = (cg + 6) * U * big / sd * (1 + z.abs()) + 12 * U * z.abs()
+    assert bool(((out.double().view(n, groups, -1) - z).abs() <= bound).all())
