@@ -73,3 +73,17 @@ def test_groups_of_few_near_values(c, groups):
     big = (v - v[:, :, :1]).abs().amax(2, keepdim=True)
     bound = (cg + 6) * U * big / sd * (1 + z.abs()) + 12 * U * z.abs()
     assert bool(((out.double().view(n, groups, -1) - z).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("c,groups", [(32, 8), (100, 25), (128, 16), (64, 16)])
+def test_equal_values_far_from_zero(c, groups):
+    """Graphs whose features are equal within a group, whole numbers up to 4,095: with counts that are powers of two every
+    sum is exact, so the deviation is 0 and the output is the bias, in graphs short and long, whole and split."""
+    lengths = torch.tensor([1, 2, 4, 8, 16, 32, 64] * 40 + [128, 256, 1024, 4096] + [1] * 30, device=DEV)
+    ptr = torch.cat([lengths.new_zeros(1), lengths.cumsum(0)])
+    per = torch.randint(1000, 4096, (len(lengths), groups), device=DEV).float()
+    x = per.repeat_interleave(lengths, 0).repeat_interleave(c // groups, 1)
+    w, b = torch.rand(c, device=DEV) + 0.5, torch.randn(c, device=DEV)
+    out = torch.empty_like(x)
+    M.group_norm_forward_(x, groups, w, b, out, graph_ptr=ptr)
+    assert torch.equal(out, b.expand_as(out))
