@@ -646,12 +646,17 @@ int launch(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int64_t k
 }
 
 // Whether the few-rows kernel takes the call: fp32 output, aligned w, and rows so small
-// together that every block can quantise them for itself. Measured against the tile
-// kernel with its quantiser (fp32 rows, us on the device): K x N = 128 x 128, 16 rows 5.0 /
-// 7.5; 512 x 512, 16 rows 8.0 / 9.0, 17 rows 10.9 / 9.0; 1024 x 4096, 8 rows 11.4 / 11.0,
-// 16 rows 20.2 / 11.0.
-bool small_call(const int8_t* w, int64_t ldw, int out_type, int64_t m, int64_t k) {
-  return out_type == GNN_ROWS_FP32 && m <= kSmallRows && (m == 1 || m * k <= 8192) &&
+// together that every block can quantise or copy them for itself, a warp a row. Measured
+// against the tile kernel (with the quantiser for fp32 rows), us on the device, K x N:
+//   fp32 rows   512 x 512, 1 row 4.6 / 8.0, 16 rows 8.0 / 8.5; 512 x 4096, 16 rows 11.9 / 8.6;
+//               1024 x 4096, 8 rows 11.2 / 10.9 (whole calls 12.7 / 18.7); 2048 x 512, 1 row 12.6 / 13.6;
+//               4096 x 512, 1 row 23.4 / 17.8; 40,960 x 512, 1 row 405 / 106
+//   8-bit rows  4096 x 512, 1 row 11.2 / 15.3, 2 rows 15.8 / 15.3; 40,960 x 512, 1 row 95.3 / 95.0
+constexpr int64_t kSmallK = 2048;  // the longest row that is quantised, or stands beside others
+
+bool small_call(int x_type, const int8_t* w, int64_t ldw, int out_type, int64_t m, int64_t k) {
+  const bool alone = m == 1 && x_type == GNN_ROWS_INT8;
+  return out_type == GNN_ROWS_FP32 && m <= kSmallRows && (alone || (k <= kSmallK && m * k <= 8192)) &&
          m * round_up(k, 16) <= kSmallBytes && aligned_rows(w, ldw);
 }
 
@@ -685,7 +690,7 @@ struct Plan {
 Plan plan_for(const void* x, int x_type, int64_t ldx, const int8_t* w, int64_t ldw, int out_type, int64_t m, int64_t k,
               int64_t n) {
   Plan p;
-  if (small_call(w, ldw, out_type, m, k)) return p;
+  if (small_call(x_type, w, ldw, out_type, m, k)) return p;
   const int64_t pitch = round_up(std::max<int64_t>(k, 1), 16);
   if (x_type == GNN_ROWS_FP32) {
     p.x_bytes = round_up(m * pitch, 256);
@@ -749,7 +754,7 @@ extern "C" int gnn_linear_int8_forward(const void* x, int x_type, int64_t ldx, c
   GNN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, GNN_ERR_WORKSPACE,
               "workspace must be 256-byte aligned");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (small_call(weight, ldw, out_type, m, k)) {
+  if (small_call(x_type, weight, ldw, out_type, m, k)) {
     const SmallParams sp{x, ldx, x_type == GNN_ROWS_FP32 ? nullptr : x_scale, weight, ldw, weight_scale, bias,
                          static_cast<float*>(out), ldo, static_cast<int>(m), static_cast<int>(k), static_cast<int>(n),
                          relu ? 1 : 0};

@@ -72,6 +72,23 @@ def test_long_k_one_column_tile():
     _check_linear(4 * 148 * 128 + 77, 1100, 200, True)
 
 
+@pytest.mark.parametrize("m,k", [(1, 2048), (1, 2049), (1, 4096), (1, 40_000), (2, 2047), (2, 4096), (4, 2049), (8, 1024)])
+def test_few_long_rows(m, k):
+    """fp32 rows beside the limits of the few-rows kernel: the bits of quantiser and 8-bit transform."""
+    _check_linear(m, k, 300, False)
+    g = torch.Generator(device=DEV).manual_seed(k)
+    x, w = torch.randn(m, k, device=DEV, generator=g), _rows8(300, k, g)
+    sw = torch.rand(300, device=DEV, generator=g) + 0.1
+    q, s = I.empty_rows(m, k, DEV), torch.empty(m, device=DEV)
+    I.quantize_rows_(x, q, s)
+    eq, es = _quantize(x)
+    assert torch.equal(q, eq) and torch.equal(s, es)
+    want, out = torch.empty(m, 300, device=DEV), torch.empty(m, 300, device=DEV)
+    I.linear_int8_forward_(q, s, w, sw, None, want)
+    I.linear_int8_forward_(x, None, w, sw, None, out)
+    assert torch.equal(out, want)
+
+
 def _check_spmm(n, nnz, f, agg, index, seed=1):
     g = torch.Generator(device=DEV).manual_seed(seed)
     # skewed degrees: hubs over many shares, rows without entries
