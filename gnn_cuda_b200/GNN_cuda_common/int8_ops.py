@@ -90,7 +90,8 @@ def _check_vector(name: str, t: torch.Tensor, length: int, index: int, what: str
         _check(False, f"{name} length must equal {what}")
 
 
-def _check_apart(out: torch.Tensor, out_ptr: int, out_ld: int, x: torch.Tensor, x_ptr: int, x_ld: int) -> None:
+def _check_apart(out: torch.Tensor, out_ptr: int, out_ld: int, x: torch.Tensor, x_ptr: int, x_ld: int,
+                 what: str = "out must not alias x") -> None:
     """Refuses an output whose address range meets that of x (matrices of contiguous rows)."""
     if out_ptr <= x_ptr:
         m, n = out.shape
@@ -99,7 +100,7 @@ def _check_apart(out: torch.Tensor, out_ptr: int, out_ld: int, x: torch.Tensor, 
         m, n = x.shape
         first, last = out_ptr, x_ptr + ((m - 1) * x_ld + n) * x.element_size()
     if first < last and out.numel() and x.numel():
-        _check(False, "out must not alias x")
+        _check(False, what)
 
 
 class _On:
@@ -145,6 +146,7 @@ def quantize_rows_(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> Non
     rows, cols = x.shape
     _check(x.shape == q.shape, "x and q must have the same shape")
     _check_vector("scale", scale, rows, index, "the number of rows")
+    _check_apart(q, q.data_ptr(), ldq, x, x.data_ptr(), cols, "q must not alias x")
     with _On(index) as stream:
         N.check(N.lib().gnn_quantize_rows(x.data_ptr(), cols, rows, cols, q.data_ptr(), ldq, scale.data_ptr(), stream),
                 "gnn_quantize_rows")
@@ -158,6 +160,7 @@ def quantize_weight_(weight: torch.Tensor, q: torch.Tensor, scale: torch.Tensor)
     k, n = weight.shape
     _check(k == q.shape[1] and n == q.shape[0], "q must be [out, in] for weight [in, out]")
     _check_vector("scale", scale, n, index, "the number of output channels")
+    _check_apart(q, q.data_ptr(), ldq, weight, weight.data_ptr(), n, "q must not alias weight")
     with _On(index) as stream:
         N.check(N.lib().gnn_quantize_weight(weight.data_ptr(), k, n, q.data_ptr(), ldq, scale.data_ptr(), stream),
                 "gnn_quantize_weight")

@@ -295,12 +295,14 @@ typedef enum gnn_row_type {
 /* scale[i] = fp32(max_j |x[i, j]| / 127); q[i, j] = x[i, j] / scale[i] rounded to
  * the nearest integer, ties to even, decided on the exact quotient. A row of zeros
  * (or whose scale underflows) has scale 0 and q 0; a row that holds a NaN or an
- * infinity has scale NaN and q 0. Bytes of q between cols and ldq are not written. */
+ * infinity has scale NaN and q 0. Bytes of q between cols and ldq are not written. q must
+ * not overlap x. */
 int gnn_quantize_rows(const float* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq,
                       float* scale, gnn_stream_t stream);
 
 /* The columns of weight [k, n] (the layout of gnn_linear_forward) as n rows of k
- * 8-bit values, one scale per output channel: q is [n, ldq], scale is [n]. */
+ * 8-bit values, one scale per output channel: q is [n, ldq], scale is [n]. q must not
+ * overlap weight. */
 int gnn_quantize_weight(const float* weight, int64_t k, int64_t n, int8_t* q, int64_t ldq, float* scale,
                         gnn_stream_t stream);
 
