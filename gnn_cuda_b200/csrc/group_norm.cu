@@ -15,9 +15,9 @@
 // per window in the workspace; a second kernel joins the pieces, a third reads x again
 // and writes. So a long graph costs three passes over its rows where x exceeds the L2.
 //
-// Measured on one B200: 232,965 nodes x 256 on their own, SiLU, 88 us = 0.83 of copy
+// Measured on one B200: 232,965 nodes x 256 on their own, SiLU, 84-88 us = 0.83 of copy
 // bandwidth; one graph of 2,449,029 x 128 602 us, three passes at 0.95 of it (joining its
-// pieces 11 us); 8,192 ragged graphs, 200,003 x 100, GELU, 114 us, bound by latency: 24
+// pieces 11 us); 8,192 ragged graphs, 200,003 x 100, GELU, 114 us (108 on the device), bound by latency: 24
 // warps an SM, each of which waits for a graph's statistics before it writes its rows.
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -16,11 +16,14 @@
 // gives as their number: that one sizes the grid and the scratch and is the length of
 // col_ind and edge_weight, so entries past it count as absent and are recorded as a status.
 //
-// Measured on one B200 (612,257 nodes, 16,077,042 entries, GCN, F = 128): 447 us and 25 us
-// for the pieces. Bound by instructions (0.66 a cycle and scheduler; unpacking and adding
+// Measured on one B200 (612,257 nodes, 16,077,042 entries, GCN, F = 128): 448 us, the pieces
+// among them. Bound by instructions (0.66 a cycle and scheduler; unpacking and adding
 // 16 columns of an entry takes 36) and by the L2's gathers (2.06 GB of rows at 4.6 TB/s).
 // Against it: a whole warp per share with four columns a lane 684-790 us, lane groups on
-// one share joined at row ends 712 us, two rows in flight instead of four 521 us.
+// one share joined at row ends 712 us, two rows in flight instead of four 521 us. The loop is
+// sensitive to registers: row ends clamped to the span in it 467 us, degrees taken from the
+// row ends 479 us, the first entry's place in 64 bits 468 us. Byte loads, of 100,000
+// contiguous rows of 100 columns with 1,500,000 entries: 175 us.
 #include <cuda_runtime.h>
 #include <stdint.h>
 

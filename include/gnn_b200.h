@@ -366,7 +366,7 @@ typedef enum gnn_activation {
  * nor written. groups = 1 normalises whole rows / graphs, groups = channels each
  * channel. At most 1024 channels per group. weight and bias may be NULL. out may be
  * x itself, else must not overlap it. Workspace: gnn_group_norm_workspace_bytes, with
- * graph_ptr only. Deterministic, no atomics. */
+ * graph_ptr only. Deterministic, no floating-point atomics. */
 size_t gnn_group_norm_workspace_bytes(int64_t num_nodes, int64_t num_graphs, int64_t groups);
 int gnn_group_norm_forward(const float* x, const void* graph_ptr, int graph_ptr_type, int64_t num_graphs,
                            const float* weight, const float* bias, float* out, int64_t num_nodes,
