@@ -17,8 +17,8 @@
 //
 // Measured on one B200: 232,965 nodes x 256 on their own, SiLU, 84-88 us = 0.83 of copy
 // bandwidth; one graph of 2,449,029 x 128 602 us, three passes at 0.95 of it (joining its
-// pieces 11 us); 8,192 ragged graphs, 200,003 x 100, GELU, 114 us (108 on the device), bound by latency: 24
-// warps an SM, each of which waits for a graph's statistics before it writes its rows.
+// pieces 11 us); 8,192 ragged graphs, 200,003 x 100, GELU, 114 us (108 on the device), bound by
+// latency: 24 warps an SM, each of which waits for a graph's statistics before it writes its rows.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -69,9 +69,8 @@ __device__ __forceinline__ float gelu(float y) {
   const float z = fminf(fabsf(y), 20.0f);
   const float p = fmaf(fmaf(fmaf(0.014852066524326801f, z, 0.11001348495483398f), z, 0.34495601058006287f), z,
                        0.4999999403953552f);
-  const float q = fmaf(
-      fmaf(fmaf(fmaf(0.037241388112306595f, z, 0.2753705382347107f), z, 0.9071747064590454f), z, 1.4877893924713135f), z,
-      1.0f);
+  const float r = fmaf(fmaf(0.037241388112306595f, z, 0.2753705382347107f), z, 0.9071747064590454f);
+  const float q = fmaf(fmaf(r, z, 1.4877893924713135f), z, 1.0f);
   return (y < 0.0f ? 0.0f : y) - z * __fdividef(p, q) * __expf(-0.5f * z * z);
 }
 
@@ -661,7 +660,9 @@ struct Team {
       for (int j = 0; j < NV; ++j) {
         if (t.live(j)) {
 #pragma unroll
-          for (int e = 0; e < CH; ++e) v[u][j][e] = activate<ACT>(fmaf(v[u][j][e] - mean[j][e % E], scale[j][e], shift[j][e]));
+          for (int e = 0; e < CH; ++e) {
+            v[u][j][e] = activate<ACT>(fmaf(v[u][j][e] - mean[j][e % E], scale[j][e], shift[j][e]));
+          }
           store_chunk<CH>(q + u * step + 32 * CH * j, v[u][j]);
         }
       }
@@ -1015,7 +1016,8 @@ int run(const NormArgs& a, bool rows, unsigned tiles, cudaStream_t s) {
     return GNN_OK;
   }
   const size_t smem = warps + sizeof(float2) * 2 * kWarps * a.tile_groups;
-  constexpr size_t most = sizeof(float) * kWarps * scratch_floats<CH, NV, WHOLE>() + sizeof(float2) * 2 * kWarps * kTile;
+  constexpr size_t most =
+      sizeof(float) * kWarps * scratch_floats<CH, NV, WHOLE>() + sizeof(float2) * 2 * kWarps * kTile;
   static_assert(most + sizeof(Window) + 1024 <= 227 * 1024, "the largest call has to fit");
   const dim3 grid(static_cast<unsigned>(a.windows), tiles);
   if (int rc = allow_shared<norm_windows_kernel<CH, NV, WHOLE>>(smem, most)) return rc;

@@ -241,7 +241,9 @@ __global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
   // (past len, so that the row ends behind the loop, where the entries are cut off)
   // (r unsigned: one past the last of 2^31 - 1 rows is no negative place)
   auto load_stop = [&](uint32_t r) -> int {
-    return r < static_cast<uint32_t>(row_end) ? static_cast<int>(__ldg(static_cast<const IdxT*>(a.row_ptr) + r + 1) - entry) : 0x7fffffff;
+    return r < static_cast<uint32_t>(row_end)
+               ? static_cast<int>(__ldg(static_cast<const IdxT*>(a.row_ptr) + r + 1) - entry)
+               : 0x7fffffff;
   };
   auto load_factor = [&](uint32_t r) -> float {
     return r < static_cast<uint32_t>(row_end) ? row_factor<IdxT>(a, r) : 0.0f;
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 4) spmm_i8_kernel(I8SpmmArgs a) {
     w_cur = w_nxt;
     c_nxt = c_far;
   }
-  for (bool any = true; row < row_end; any = false) finish_row(any);               // rows that end with the share's last entry
+  for (bool any = true; row < row_end; any = false) finish_row(any);  // rows that end with the share's last entry
   if (open) store(head ? partl : partl + a.f, 1.0f);  // entries of a row that ends in a later share
 }
 

@@ -77,8 +77,8 @@ def test_groups_of_few_near_values(c, groups):
 
 @pytest.mark.parametrize("c,groups", [(32, 8), (100, 25), (128, 16), (64, 16)])
 def test_equal_values_far_from_zero(c, groups):
-    """Graphs whose features are equal within a group, whole numbers up to 4,095: with counts that are powers of two every
-    sum is exact, so the deviation is 0 and the output is the bias, in graphs short and long, whole and split."""
+    """Graphs whose features are equal within a group, whole numbers up to 4,095: with counts that are powers of two
+    every sum is exact, so the deviation is 0 and the output is the bias, in graphs short and long, whole and split."""
     lengths = torch.tensor([1, 2, 4, 8, 16, 32, 64] * 40 + [128, 256, 1024, 4096] + [1] * 30, device=DEV)
     ptr = torch.cat([lengths.new_zeros(1), lengths.cumsum(0)])
     per = torch.randint(1000, 4096, (len(lengths), groups), device=DEV).float()

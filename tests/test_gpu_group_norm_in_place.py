@@ -26,6 +26,7 @@ def test_batches(c, groups, low, high, graphs):
     _check(torch.randn(int(ptr[-1]) + 70, c, device=DEV), groups, ptr)
 
 
-@pytest.mark.parametrize("n,c,groups", [(50_001, 27, 3), (30_000, 32, 32), (7_000, 300, 100), (20_000, 256, 16), (9, 5, 1)])
+@pytest.mark.parametrize("n,c,groups", [(50_001, 27, 3), (30_000, 32, 32), (7_000, 300, 100), (20_000, 256, 16),
+                                        (9, 5, 1)])
 def test_nodes(n, c, groups):
     _check(torch.randn(n, c, device=DEV), groups, None)

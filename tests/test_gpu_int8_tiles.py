@@ -72,7 +72,8 @@ def test_long_k_one_column_tile():
     _check_linear(4 * 148 * 128 + 77, 1100, 200, True)
 
 
-@pytest.mark.parametrize("m,k", [(1, 2048), (1, 2049), (1, 4096), (1, 40_000), (2, 2047), (2, 4096), (4, 2049), (8, 1024)])
+@pytest.mark.parametrize("m,k", [(1, 2048), (1, 2049), (1, 4096), (1, 40_000), (2, 2047), (2, 4096), (4, 2049),
+                                 (8, 1024)])
 def test_few_long_rows(m, k):
     """fp32 rows beside the limits of the few-rows kernel: the bits of quantiser and 8-bit transform."""
     _check_linear(m, k, 300, False)
